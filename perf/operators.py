@@ -82,7 +82,7 @@ def draw(rng):
         width = _log(rng, 64, 8192)
         width -= width % rng.choice([1, 8, 64])
         stream = rng.choice(["bf16", "f16", "f32"])
-        rows = _log(rng, 1, 60_000_000 // width)
+        rows = _log(rng, 1, 28_000_000 // width)
         return _norm("drawn", rows, width, rng.choice(["rms", "layer"]), stream,
                      stream if stream != "f32" else rng.choice(["bf16", "f16", "f32"]),
                      rng.choice(["none", "linear", "sigmoid", "tanh"]), rng.choice([1, rng.randint(2, 500), rows]))
