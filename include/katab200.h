@@ -250,6 +250,123 @@ KB_API int kb_attention(const uint16_t* qkv, const float* rope_cos, const float*
 KB_API int kb_attention_amax(const uint16_t* qkv, uint16_t* out, uint32_t* row_amax, int batch, int heads,
                              int head_dim, float scale, int dtype, uintptr_t stream);
 
+/* ------------------------------------------------------------------ block operators */
+
+/* Operators of a differential-attention block over boards and their history:
+ * rotary positions with several axes, differential attention and the norms
+ * around a block.  They work on any number of tokens and any (element)
+ * strides with a contiguous innermost dimension.  Calls with nothing to do
+ * (no tokens, no rows, batch 0) succeed and launch nothing.  No reference
+ * counterparts: the reference's trunk has one softmax map over 361 tokens,
+ * rotary tables over two axes and a plain pre-norm residual. */
+
+/* Pairs that a rotation mixes, of the first 2 * pairs elements of a head. */
+#define KB_ROPE_PAIRS 0  /* (2p, 2p + 1): the trunk's own layout */
+#define KB_ROPE_HALVES 1 /* (p, p + pairs) */
+
+/* Rotary positions with several axes: for every token t, head h < rotary_heads
+ * and pair p < pairs, with angle = sum_a positions[a, t] * freqs[h, p, a],
+ *   (u, v) -> (u cos - v sin, u sin + v cos);
+ * every other element is copied.  x: [tokens, heads, head_dim] of dtype
+ * KB_DT_*, strides x_token / x_head; positions int32 [axes, tokens], axes
+ * 1..4; freqs fp32 [freq_heads, pairs, axes] with freq_heads 1 (shared) or
+ * rotary_heads; out has x's type, strides out_token / out_head.  A frequency
+ * table with one nonzero axis per pair gives the sectioned form (time, height,
+ * width); two axes with learned frequencies are the trunk's.  The angle is
+ * summed and reduced to one turn in 64 bits, so long positions cost no accuracy.
+ * slots (nullable, int64 [tokens]): token t goes to row slots[t] of out instead
+ * of row t; rows outside [0, out_rows) are not written (out_rows is ignored
+ * without slots).  out may be x with the same strides and no slots; any other
+ * overlap of the two is the caller's error. */
+KB_API int kb_rope_axes(const void* x, int dtype, int tokens, int heads, int head_dim, int64_t x_token, int64_t x_head,
+                        const int32_t* positions, int axes, const float* freqs, int freq_heads, int pairs,
+                        int rotary_heads, int layout, const int64_t* slots, int64_t out_rows, void* out,
+                        int64_t out_token, int64_t out_head, uintptr_t stream);
+
+#define KB_NORM_NONE 0
+#define KB_NORM_RMS 1   /* v / sqrt(mean(v^2) + eps) * gamma + beta */
+#define KB_NORM_LAYER 2 /* (v - mean) / sqrt(var + eps) * gamma + beta */
+
+#define KB_GATE_LINEAR 0
+#define KB_GATE_SIGMOID 1
+#define KB_GATE_TANH 2
+
+/* The norms around a block: one pass over the residual stream x and the
+ * block's output y,
+ *   r = res_scale * x + branch_scale * gate_act(gate) * post_norm(y)
+ *   h = pre_norm(r) * (1 + mod_scale) + mod_shift
+ * r is written to x_out rounded to the stream's type, h (the next block's
+ * input) is computed from the unrounded r.  Statistics in fp32. */
+typedef struct kb_norm_residual_desc {
+  int rows, width;      /* width 1..16384 */
+  int stream_dtype;     /* x, x_out: KB_DT_* */
+  int branch_dtype;     /* y, h, gate, mod_scale, mod_shift: KB_DT_* */
+  int post_norm;        /* KB_NORM_* of y */
+  int pre_norm;         /* KB_NORM_* of r */
+  int gate_act;         /* KB_GATE_* */
+  int rows_per_cond;    /* rows that share one row of gate, mod_scale and mod_shift: row / rows_per_cond */
+  float res_scale, branch_scale, eps;
+  int64_t x_stride, y_stride, x_out_stride, h_stride, cond_stride; /* row strides in elements */
+} kb_norm_residual_desc;
+
+/* y, gate, mod_scale, mod_shift, the gammas and the betas (fp32 [width]) may be
+ * NULL (y: r = res_scale * x; gate: 1; mods: 0; gamma: 1; beta: 0); x_out or h
+ * may be NULL when it is not wanted, not both.  x_out may be x, and h may be y,
+ * with the same stride. */
+KB_API int kb_norm_residual(const kb_norm_residual_desc* desc, const void* x, const void* y, const float* post_gamma,
+                            const float* post_beta, const float* pre_gamma, const float* pre_beta, const void* gate,
+                            const void* mod_scale, const void* mod_shift, void* x_out, void* h, uintptr_t stream);
+
+/* Differential attention: with s = scale, for every query i and head h, whose
+ * keys and values are those of head h / (heads / kv_heads),
+ *   o = softmax(s q1 K1^T) V - lambda_h softmax(s q2 K2^T) V
+ *   out = out_scale * gamma * o / sqrt(mean(o^2) + eps)    (o * out_scale if gamma is NULL)
+ * q [batch, q_len, heads, 2, head_dim], k [batch, kv_len, kv_heads, 2,
+ * head_dim], v [batch, kv_len, kv_heads, 2 * head_dim], out [batch, q_len,
+ * heads, 2 * head_dim], all of dtype KB_DT_F16 or KB_DT_BF16.
+ * Keys: those below kv_lens[b] (nullable, int32 [batch], clamped to [0,
+ * kv_len]) whose key_mask byte (nullable, [batch, kv_len], row stride
+ * mask_batch) is nonzero.  causal: query i of a sequence of n keys sits at
+ * position n - q_len + i and sees the keys up to there, with window > 0 only
+ * the last `window` of them.  A query that sees no key gets zeros.  What lies
+ * in K and V at keys that kv_lens or key_mask hide is never used, NaN and
+ * infinities included; a non-finite value of V at a key that only the causal
+ * mask or the window hides may reach other queries of the call. */
+typedef struct kb_diff_attention_desc {
+  int dtype;           /* KB_DT_F16 or KB_DT_BF16 */
+  int batch, q_len, kv_len;
+  int heads, kv_heads; /* heads a multiple of kv_heads */
+  int head_dim;        /* 32 or 64: of each map; values and outputs are twice as wide */
+  int causal, window;  /* window 0: none; needs causal */
+  float scale, out_scale, eps;
+  /* strides in elements, multiples of 8 (dimensions of extent 1: ignored); the
+   * base addresses are 16-byte aligned */
+  int64_t q_batch, q_token, q_head, q_map;
+  int64_t k_batch, k_token, k_head, k_map;
+  int64_t v_batch, v_token, v_head;
+  int64_t out_batch, out_token, out_head;
+  int64_t mask_batch; /* bytes, any */
+} kb_diff_attention_desc;
+
+/* Bytes of device scratch that kb_diff_attention needs for this descriptor (0
+ * when it splits nothing over the keys).  Calls that overlap on the GPU must
+ * not share it; nothing in it needs clearing between calls. */
+KB_API int kb_diff_attention_workspace(const kb_diff_attention_desc* desc, size_t* bytes);
+
+/* lambda: fp32 [heads]; gamma: fp32 [2 * head_dim] or NULL; status: a status
+ * word (nullable) that receives KB_STATUS_TIMEOUT if a bounded wait gave up.
+ * workspace: 16-byte aligned, at least kb_diff_attention_workspace bytes. */
+KB_API int kb_diff_attention(const kb_diff_attention_desc* desc, const uint16_t* q, const uint16_t* k,
+                             const uint16_t* v, const float* lambda, const float* gamma, const int32_t* kv_lens,
+                             const uint8_t* key_mask, uint16_t* out, void* workspace, size_t workspace_bytes,
+                             uint32_t* status, uintptr_t stream);
+
+/* The maps' weight of each head from its learned vectors (CPU, load time; fp32
+ * [heads, head_dim] host arrays, sums in fp64):
+ *   lambda_h = exp(q1_h . k1_h) - exp(q2_h . k2_h) + lambda_init */
+KB_API int kb_diff_lambda(const float* q1, const float* k1, const float* q2, const float* k2, int heads, int head_dim,
+                          float lambda_init, float* lambda);
+
 /* ------------------------------------------------------------------ MXFP8 (block-scaled E4M3) */
 
 /* Status word [flags, first_layer]: flags OR-ed, first_layer = first layer

@@ -15,6 +15,7 @@ P = ctypes.c_void_p
 I = ctypes.c_int
 F = ctypes.c_float
 U = ctypes.c_uint64
+L = ctypes.c_int64
 PP = ctypes.POINTER(ctypes.c_void_p)
 IP = ctypes.POINTER(ctypes.c_int)
 STREAM = ctypes.c_size_t  # uintptr_t
@@ -47,6 +48,11 @@ SIGNATURES: dict[str, tuple] = {
     "kb_f16_linear": (I, [P, P, P, I, I, I, I, I, I, P, I, STREAM]),
     "kb_attention": (I, [P, P, P, P, I, I, I, F, I, STREAM]),
     "kb_attention_amax": (I, [P, P, P, I, I, I, F, I, STREAM]),
+    "kb_rope_axes": (I, [P, I, I, I, I, L, L, P, I, P, I, I, I, I, P, L, P, L, L, STREAM]),
+    "kb_norm_residual": (I, [P, P, P, P, P, P, P, P, P, P, P, P, STREAM]),
+    "kb_diff_attention_workspace": (I, [P, ctypes.POINTER(ctypes.c_size_t)]),
+    "kb_diff_attention": (I, [P, P, P, P, P, P, P, P, P, P, ctypes.c_size_t, P, STREAM]),
+    "kb_diff_lambda": (I, [P, P, P, P, I, I, F, P]),
     "kb_status_reset": (I, [P, STREAM]),
     "kb_mxfp8_dimensions": (I, [I, I, IP, IP, ctypes.POINTER(ctypes.c_size_t), ctypes.POINTER(ctypes.c_size_t)]),
     "kb_mxfp8_quantize": (I, [P, I, I, I, I, P, P, ctypes.c_size_t, P, ctypes.c_uint32, STREAM]),
@@ -112,6 +118,25 @@ class PostProcessParams(ctypes.Structure):
         return cls(**dict(cls.DEFAULTS, **kw))
 
 
+class NormResidualDesc(ctypes.Structure):
+    """kb_norm_residual_desc."""
+
+    _fields_ = [(n, I) for n in ("rows", "width", "stream_dtype", "branch_dtype", "post_norm", "pre_norm", "gate_act",
+                                 "rows_per_cond")]
+    _fields_ += [(n, F) for n in ("res_scale", "branch_scale", "eps")]
+    _fields_ += [(n, L) for n in ("x_stride", "y_stride", "x_out_stride", "h_stride", "cond_stride")]
+
+
+class DiffAttentionDesc(ctypes.Structure):
+    """kb_diff_attention_desc."""
+
+    _fields_ = [(n, I) for n in ("dtype", "batch", "q_len", "kv_len", "heads", "kv_heads", "head_dim", "causal",
+                                 "window")]
+    _fields_ += [(n, F) for n in ("scale", "out_scale", "eps")]
+    _fields_ += [(n, L) for n in ("q_batch", "q_token", "q_head", "q_map", "k_batch", "k_token", "k_head", "k_map",
+                                  "v_batch", "v_token", "v_head", "out_batch", "out_token", "out_head", "mask_batch")]
+
+
 # Constants mirrored from include/katab200.h.
 KB_OK, KB_E_INVALID, KB_E_CUDA, KB_E_STATE, KB_E_NONFINITE, KB_E_UNSUPPORTED = range(6)
 PROJ_FOLLOW, PROJ_INT8, PROJ_MXFP8, PROJ_BF16 = range(4)
@@ -121,6 +146,9 @@ ACT_NONE, ACT_GELU, ACT_SILU = 0, 1, 2
 LAYOUT_PLAIN, LAYOUT_SWIGLU_DUAL = 0, 1
 PREC_INT8, PREC_MXFP8 = 0, 1
 TOPO_FLAT, TOPO_NESTED = 0, 1
+ROPE_PAIRS, ROPE_HALVES = 0, 1
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
+GATE_LINEAR, GATE_SIGMOID, GATE_TANH = 0, 1, 2
 MX_OUT_HALF, MX_OUT_FLOAT, MX_OUT_FLOAT_RESIDUAL, MX_OUT_BF16, MX_OUT_BF16_RESIDUAL = range(5)
 STATUS_NAN, STATUS_INF, STATUS_OUTPUT_NONFINITE, STATUS_WEIGHT_OVERFLOW = 1, 2, 4, 8
 STATUS_UNSUPPORTED_ARCH, STATUS_TIMEOUT = 16, 32

@@ -1,0 +1,181 @@
+// Differential attention (kb_diff_attention): the difference of two softmax
+// maps over shared values,
+//   o = softmax(s q1 K1^T) V - lambda softmax(s q2 K2^T) V,
+// then out = out_scale * gamma * o / sqrt(mean(o^2) + eps).
+#include <math.h>
+#include <stdint.h>
+
+#include "kb_diff.cuh"
+#include "kb_internal.h"
+#include "kb_numeric.cuh"
+
+namespace kb {
+namespace {
+
+// One warp per (batch, head, query); lanes take one key each for the two dot
+// products and the running maxima and sums, then 2D / 32 dims each of the two
+// value sums.
+template <int D>
+__global__ void __launch_bounds__(128) diff_simple_kernel(const DiffArgs a) {
+  constexpr int kDims = 2 * D / 32;
+  __shared__ float qs[4][2 * D];
+  const kb_diff_attention_desc& d = a.d;
+  const bool f16 = d.dtype == KB_DT_F16;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t job = static_cast<int64_t>(blockIdx.x) * 4 + warp;
+  if (job >= static_cast<int64_t>(d.batch) * d.heads * d.q_len) return;
+  const int i = static_cast<int>(job % d.q_len);
+  const int h = static_cast<int>(job / d.q_len % d.heads);
+  const int b = static_cast<int>(job / d.q_len / d.heads);
+  const int hk = h / (d.heads / d.kv_heads);
+  for (int c = lane; c < 2 * D; c += 32)
+    qs[warp][c] = from16(a.q[b * d.q_batch + i * d.q_token + h * d.q_head + (c / D) * d.q_map + c % D], f16);
+  __syncwarp();
+  int first, last;
+  key_range(a, b, i, i, first, last);
+  const uint16_t* k0 = a.k + b * d.k_batch + hk * d.k_head;
+  const uint16_t* v0 = a.v + b * d.v_batch + hk * d.v_head;
+  const uint8_t* mask = a.key_mask ? a.key_mask + b * d.mask_batch : nullptr;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[2][kDims] = {};
+  for (int j0 = first; j0 < last; j0 += 32) {
+    const int j = j0 + lane;
+    const bool see = j < last && (!mask || mask[j]);
+    float p[2];
+    for (int t = 0; t < 2; ++t) {
+      float s = -INFINITY;
+      if (see) {
+        const uint16_t* kr = k0 + j * d.k_token + t * d.k_map;
+        s = 0.0f;
+        for (int c = 0; c < D; ++c) s = fmaf(qs[warp][t * D + c], from16(kr[c], f16), s);
+        s *= a.scale_log2;
+      }
+      float mt = s;
+      for (int x = 16; x; x >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, x));
+      const float mn = fmaxf(m[t], mt);
+      const float base = mn == -INFINITY ? 0.0f : mn;
+      const float f = exp2f(m[t] - base);
+      p[t] = exp2f(s - base);
+      m[t] = mn;
+      l[t] = l[t] * f + p[t];
+      for (int c = 0; c < kDims; ++c) o[t][c] *= f;
+    }
+    for (int u = 0; u < 32; ++u) {
+      const float p0 = __shfl_sync(0xffffffffu, p[0], u), p1 = __shfl_sync(0xffffffffu, p[1], u);
+      const bool use = __shfl_sync(0xffffffffu, static_cast<int>(see), u);
+      if (!use) continue;
+      for (int c = 0; c < kDims; ++c) {
+        const float v = from16(v0[(j0 + u) * d.v_token + c * 32 + lane], f16);
+        o[0][c] = fmaf(p0, v, o[0][c]);
+        o[1][c] = fmaf(p1, v, o[1][c]);
+      }
+    }
+  }
+  for (int t = 0; t < 2; ++t)
+    for (int x = 16; x; x >>= 1) l[t] += __shfl_xor_sync(0xffffffffu, l[t], x);
+  const float w0 = m[0] == -INFINITY ? 0.0f : 1.0f / l[0];
+  const float w1 = m[1] == -INFINITY ? 0.0f : a.lambda[h] / l[1];
+  float ss = 0.0f, r[kDims];
+  for (int c = 0; c < kDims; ++c) {
+    r[c] = o[0][c] * w0 - o[1][c] * w1;
+    ss = fmaf(r[c], r[c], ss);
+  }
+  for (int x = 16; x; x >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, x);
+  const float rstd = a.gamma ? 1.0f / sqrtf(ss / (2 * D) + d.eps) : 1.0f;
+  uint16_t* out = a.out + b * d.out_batch + i * d.out_token + h * d.out_head;
+  for (int c = 0; c < kDims; ++c) {
+    const float g = a.gamma ? a.gamma[c * 32 + lane] : 1.0f;
+    out[c * 32 + lane] = bits16(r[c] * rstd * g * d.out_scale, f16);
+  }
+}
+
+int bad(const char* what) {
+  set_error(std::string("kb_diff_attention: ") + what);
+  return KB_E_INVALID;
+}
+
+int check_desc(const kb_diff_attention_desc* desc) {
+  if (!desc) return bad("null descriptor");
+  const kb_diff_attention_desc& d = *desc;
+  if (d.dtype != KB_DT_F16 && d.dtype != KB_DT_BF16) return bad("dtype must be KB_DT_F16 or KB_DT_BF16");
+  if (d.head_dim != 32 && d.head_dim != 64) return bad("head_dim must be 32 or 64");
+  if (d.batch < 0 || d.q_len < 0 || d.kv_len < 0) return bad("batch, q_len and kv_len must not be negative");
+  if (d.batch > 65535 || d.q_len > (1 << 26) || d.kv_len > (1 << 30) || d.heads > 1024)
+    return bad("at most 65535 sequences, 2^26 queries, 2^30 keys and 1024 heads");
+  if (d.heads < 1 || d.kv_heads < 1 || d.heads % d.kv_heads) return bad("heads must be a multiple of kv_heads");
+  if (d.window < 0 || (d.window > 0 && !d.causal)) return bad("a window must be positive and causal");
+  if (!isfinite(d.scale) || !isfinite(d.out_scale) || !(d.eps >= 0.0f)) return bad("scale, out_scale or eps");
+  const int64_t most = int64_t(1) << 38;
+  auto ok = [&](int64_t stride, int64_t extent) { return extent <= 1 || (stride >= 0 && stride < most && stride % 8 == 0); };
+  if (!ok(d.q_batch, d.batch) || !ok(d.q_token, d.q_len) || !ok(d.q_head, d.heads) || !ok(d.q_map, 2) ||
+      !ok(d.k_batch, d.batch) || !ok(d.k_token, d.kv_len) || !ok(d.k_head, d.kv_heads) || !ok(d.k_map, 2) ||
+      !ok(d.v_batch, d.batch) || !ok(d.v_token, d.kv_len) || !ok(d.v_head, d.kv_heads) ||
+      !ok(d.out_batch, d.batch) || !ok(d.out_token, d.q_len) || !ok(d.out_head, d.heads))
+    return bad("strides must be multiples of 8 elements, not negative and below 2^38");
+  auto apart = [&](int64_t stride, int64_t extent) { return extent <= 1 || stride >= 2 * d.head_dim; };
+  if (!apart(d.out_batch, d.batch) || !apart(d.out_token, d.q_len) || !apart(d.out_head, d.heads))
+    return bad("out's rows must not overlap");
+  if (d.mask_batch < 0 || d.mask_batch > most) return bad("mask_batch");
+  return KB_OK;
+}
+
+}  // namespace
+}  // namespace kb
+
+extern "C" int kb_diff_attention_workspace(const kb_diff_attention_desc* desc, size_t* bytes) {
+  using namespace kb;
+  const int rc = check_desc(desc);
+  if (rc) return rc;
+  if (!bytes) return bad("null bytes");
+  *bytes = 0;
+  return KB_OK;
+}
+
+extern "C" int kb_diff_attention(const kb_diff_attention_desc* desc, const uint16_t* q, const uint16_t* k,
+                                 const uint16_t* v, const float* lambda, const float* gamma, const int32_t* kv_lens,
+                                 const uint8_t* key_mask, uint16_t* out, void* workspace, size_t workspace_bytes,
+                                 uint32_t* status, uintptr_t stream) {
+  using namespace kb;
+  (void)status;
+  const int rc = check_desc(desc);
+  if (rc) return rc;
+  const kb_diff_attention_desc& d = *desc;
+  if (d.batch == 0 || d.q_len == 0) return KB_OK;
+  if (!q || !lambda || !out || (d.kv_len > 0 && (!k || !v))) return bad("null pointer");
+  for (const void* p : {static_cast<const void*>(q), static_cast<const void*>(k), static_cast<const void*>(v),
+                        static_cast<const void*>(out), static_cast<const void*>(workspace)})
+    if (reinterpret_cast<uintptr_t>(p) % 16) return bad("q, k, v, out and workspace must be 16-byte aligned");
+  if (out == q || out == k || out == v) return bad("out must not be an input");
+  size_t need = 0;
+  kb_diff_attention_workspace(desc, &need);
+  if (need > workspace_bytes || (need && !workspace)) {
+    set_error("kb_diff_attention: workspace of " + std::to_string(need) + " bytes needed");
+    return KB_E_INVALID;
+  }
+  const DiffArgs a = make_diff_args(d, q, k, v, lambda, gamma, kv_lens, key_mask, out);
+  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const int64_t jobs = static_cast<int64_t>(d.batch) * d.heads * d.q_len;
+  if ((jobs + 3) / 4 > 0x7fffffff) return bad("too many queries");
+  const unsigned grid = static_cast<unsigned>((jobs + 3) / 4);
+  if (d.head_dim == 64) diff_simple_kernel<64><<<grid, 128, 0, s>>>(a);
+  else diff_simple_kernel<32><<<grid, 128, 0, s>>>(a);
+  return check_cuda(cudaGetLastError(), "differential attention launch");
+}
+
+extern "C" int kb_diff_lambda(const float* q1, const float* k1, const float* q2, const float* k2, int heads,
+                              int head_dim, float lambda_init, float* lambda) {
+  using namespace kb;
+  if (!q1 || !k1 || !q2 || !k2 || !lambda || heads < 1 || head_dim < 1) {
+    set_error("kb_diff_lambda: null pointer or empty shape");
+    return KB_E_INVALID;
+  }
+  for (int h = 0; h < heads; ++h) {
+    double s1 = 0.0, s2 = 0.0;
+    for (int c = 0; c < head_dim; ++c) {
+      const int64_t at = static_cast<int64_t>(h) * head_dim + c;
+      s1 += static_cast<double>(q1[at]) * k1[at];
+      s2 += static_cast<double>(q2[at]) * k2[at];
+    }
+    lambda[h] = static_cast<float>(exp(s1) - exp(s2) + lambda_init);
+  }
+  return KB_OK;
+}

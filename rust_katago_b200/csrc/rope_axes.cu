@@ -1,0 +1,257 @@
+// Rotary positions with several axes (kb_rope_axes).
+//
+// For token t, head h and pair p the angle is sum_a pos[a, t] * freq[h, p, a];
+// the pair (u, v) becomes (u cos - v sin, u sin + v cos).
+//
+// The operator only has to read and write each element once, so HBM bounds it.
+// Each thread owns one group of VE pairs of one head for many tokens: its
+// frequencies stay in registers and nothing is shared between threads.
+// Computing sine and cosine anew for every head costs less than a table would:
+// the fp64 pipe (64 per clock and SM) does the sum over the axes and the
+// reduction to one turn exactly where fp32 would lose the low bits of long
+// positions (30,000 x a frequency of 1 already costs 1e-3 of a turn), about 5
+// operations per pair.
+#include <stdint.h>
+
+#include "kb_internal.h"
+#include "kb_numeric.cuh"
+
+namespace kb {
+namespace {
+
+struct RopeArgs {
+  const void* x;
+  const int32_t* positions;
+  const float* freqs;
+  const int64_t* slots;
+  void* out;
+  int64_t x_token, x_head, out_token, out_head, out_rows;
+  int tokens, head_dim, pairs, rotary_heads, items, per_head, freq_head_stride, f16, tokens_per_thread;
+};
+
+constexpr double kInvTwoPi = 0.15915494309189533576888;
+constexpr float kTwoPi = 6.28318530717958647692f;
+
+// cos and sin of `turns` full turns, |turns| <= 1/2.  16-bit results: the
+// special-function unit on a reduced angle (absolute error about 2^-21, far
+// below their rounding); fp32 results: CUDA's sincospif.
+template <bool WIDE>
+__device__ __forceinline__ void cos_sin_turns(float turns, float& c, float& s) {
+  if constexpr (WIDE) {
+    sincospif(2.0f * turns, &s, &c);
+  } else {
+    __sincosf(turns * kTwoPi, &s, &c);
+  }
+}
+
+// VE elements at p as floats.  ALIGNED: one 8- (16-bit) or 16-byte (fp32) load.
+template <typename T, int VE>
+struct Raw;
+template <>
+struct Raw<uint16_t, 4> { using type = uint2; };
+template <>
+struct Raw<float, 4> { using type = uint4; };
+template <>
+struct Raw<uint16_t, 1> { using type = uint16_t; };
+template <>
+struct Raw<float, 1> { using type = float; };
+
+template <typename T, int VE>
+__device__ __forceinline__ void unpack(const typename Raw<T, VE>::type& raw, bool f16, float (&v)[VE]) {
+  const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+  for (int i = 0; i < VE; ++i) {
+    if constexpr (sizeof(T) == 2) v[i] = from16(e[i], f16);
+    else v[i] = e[i];
+  }
+}
+
+template <typename T, int VE>
+__device__ __forceinline__ typename Raw<T, VE>::type pack(const float (&v)[VE], bool f16) {
+  typename Raw<T, VE>::type raw;
+  T* e = reinterpret_cast<T*>(&raw);
+#pragma unroll
+  for (int i = 0; i < VE; ++i) {
+    if constexpr (sizeof(T) == 2) e[i] = bits16(v[i], f16);
+    else e[i] = v[i];
+  }
+  return raw;
+}
+
+// A thread's item: 2 VE elements of one head, VE of them at o0 and VE at o1.
+// KB_ROPE_HALVES: u at o0 and v at o1 for pairs o0..; KB_ROPE_PAIRS: the pairs
+// o0/2.. lie interleaved across both.  VE = 1 takes any alignment.
+template <typename T, int VE, bool HALVES, int AXES>
+__global__ void __launch_bounds__(512) rope_axes_kernel(const RopeArgs a) {
+  constexpr int kUnroll = 4;
+  using R = typename Raw<T, VE>::type;
+  const int item = blockIdx.x * blockDim.x + threadIdx.x;
+  if (item >= a.items) return;
+  const int head = item / a.per_head, c = item - head * a.per_head;
+  const bool f16 = a.f16;
+  int o0 = 2 * VE * c, o1 = o0 + VE, rotated = 0;  // rotated: pairs of this item that turn
+  if (head < a.rotary_heads) {
+    if constexpr (HALVES) {
+      if (c * VE < a.pairs) {
+        o0 = c * VE;
+        o1 = a.pairs + o0;
+        rotated = VE;
+      }
+    } else {
+      rotated = max(0, min(VE, a.pairs - c * VE));
+    }
+  }
+  double freq[VE][AXES];
+  if (rotated) {
+    const float* f = a.freqs + static_cast<int64_t>(head) * a.freq_head_stride + c * VE * AXES;
+#pragma unroll
+    for (int p = 0; p < VE; ++p)
+#pragma unroll
+      for (int x = 0; x < AXES; ++x) freq[p][x] = p < rotated ? static_cast<double>(f[p * AXES + x]) * kInvTwoPi : 0.0;
+  }
+  const T* src = static_cast<const T*>(a.x) + head * a.x_head;
+  T* dst = static_cast<T*>(a.out) + head * a.out_head;
+  const int step = blockDim.y;
+  int t0 = static_cast<int>(blockIdx.y) * step * a.tokens_per_thread + threadIdx.y;
+  const int end = min(static_cast<int64_t>(a.tokens), static_cast<int64_t>(t0) + static_cast<int64_t>(step) * a.tokens_per_thread);
+  for (; t0 < end; t0 += kUnroll * step) {
+    R lo[kUnroll], hi[kUnroll];
+    int pos[kUnroll][AXES];
+    int64_t row[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int t = t0 + u * step;
+      row[u] = -1;
+      if (t < end) {
+        lo[u] = *reinterpret_cast<const R*>(src + t * a.x_token + o0);
+        hi[u] = *reinterpret_cast<const R*>(src + t * a.x_token + o1);
+#pragma unroll
+        for (int x = 0; x < AXES; ++x) pos[u][x] = rotated ? a.positions[static_cast<int64_t>(x) * a.tokens + t] : 0;
+        row[u] = t;
+        if (a.slots) {
+          row[u] = a.slots[t];
+          if (row[u] >= a.out_rows) row[u] = -1;
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      if (row[u] < 0) continue;
+      R w0 = lo[u], w1 = hi[u];
+      if (rotated) {
+        float v0[VE], v1[VE];
+        unpack<T, VE>(lo[u], f16, v0);
+        unpack<T, VE>(hi[u], f16, v1);
+#pragma unroll
+        for (int p = 0; p < VE; ++p) {
+          double turns = 0.0;
+#pragma unroll
+          for (int x = 0; x < AXES; ++x) turns = fma(static_cast<double>(pos[u][x]), freq[p][x], turns);
+          float cs, sn;
+          cos_sin_turns<sizeof(T) == 4>(static_cast<float>(turns - rint(turns)), cs, sn);
+          // element indices of the pair (u, v) in the concatenation [v0 | v1]
+          float* pu = HALVES || 2 * p < VE ? &v0[HALVES ? p : (2 * p) % VE] : &v1[(2 * p) % VE];
+          float* pv = HALVES ? &v1[p] : 2 * p + 1 < VE ? &v0[(2 * p + 1) % VE] : &v1[(2 * p + 1) % VE];
+          const float x0 = *pu, x1 = *pv;
+          const bool turn = p < rotated;  // the rest is copied, NaN and infinities too
+          *pu = turn ? x0 * cs - x1 * sn : x0;
+          *pv = turn ? x0 * sn + x1 * cs : x1;
+        }
+        w0 = pack<T, VE>(v0, f16);
+        w1 = pack<T, VE>(v1, f16);
+      }
+      *reinterpret_cast<R*>(dst + row[u] * a.out_token + o0) = w0;
+      *reinterpret_cast<R*>(dst + row[u] * a.out_token + o1) = w1;
+    }
+  }
+}
+
+template <typename T, int VE, bool HALVES>
+int launch(RopeArgs a, int heads, int axes, cudaStream_t stream) {
+  a.per_head = a.head_dim / (2 * VE);
+  a.items = heads * a.per_head;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const int nbx = (a.items + 511) / 512;
+  const int bx = ((a.items + nbx - 1) / nbx + 31) / 32 * 32;
+  const int by = bx >= 256 ? 1 : 256 / bx;
+  // Tokens per thread: enough to reuse its frequencies, few enough that every
+  // SM gets several blocks.
+  const int64_t groups = (static_cast<int64_t>(a.tokens) + by - 1) / by;
+  int64_t tpt = groups * nbx / (16 * num_sms(dev));
+  tpt = tpt < 1 ? 1 : tpt > 16 ? 16 : tpt;
+  int64_t gy = (groups + tpt - 1) / tpt;
+  if (gy > 65535) {
+    tpt = (groups + 65534) / 65535;
+    gy = (groups + tpt - 1) / tpt;
+  }
+  a.tokens_per_thread = static_cast<int>(tpt);
+  const dim3 grid(nbx, static_cast<unsigned>(gy)), block(bx, by);
+  switch (axes) {
+    case 1: rope_axes_kernel<T, VE, HALVES, 1><<<grid, block, 0, stream>>>(a); break;
+    case 2: rope_axes_kernel<T, VE, HALVES, 2><<<grid, block, 0, stream>>>(a); break;
+    case 3: rope_axes_kernel<T, VE, HALVES, 3><<<grid, block, 0, stream>>>(a); break;
+    default: rope_axes_kernel<T, VE, HALVES, 4><<<grid, block, 0, stream>>>(a); break;
+  }
+  return check_cuda(cudaGetLastError(), "rope launch");
+}
+
+int bad(const char* what) {
+  set_error(std::string("kb_rope_axes: ") + what);
+  return KB_E_INVALID;
+}
+
+}  // namespace
+}  // namespace kb
+
+extern "C" int kb_rope_axes(const void* x, int dtype, int tokens, int heads, int head_dim, int64_t x_token,
+                            int64_t x_head, const int32_t* positions, int axes, const float* freqs, int freq_heads,
+                            int pairs, int rotary_heads, int layout, const int64_t* slots, int64_t out_rows, void* out,
+                            int64_t out_token, int64_t out_head, uintptr_t stream) {
+  using namespace kb;
+  if (dtype != KB_DT_F32 && dtype != KB_DT_F16 && dtype != KB_DT_BF16) return bad("dtype must be KB_DT_*");
+  if (tokens < 0 || heads < 1 || heads > 65536 || head_dim < 2 || head_dim % 2 || head_dim > 1024)
+    return bad("tokens >= 0, heads 1..65536 and an even head_dim 2..1024 expected");
+  if (axes < 1 || axes > 4) return bad("axes must be 1..4");
+  if (pairs < 1 || 2 * pairs > head_dim) return bad("pairs must be 1..head_dim/2");
+  if (rotary_heads < 0 || rotary_heads > heads) return bad("rotary_heads must be 0..heads");
+  if (freq_heads != 1 && freq_heads != rotary_heads) return bad("freq_heads must be 1 or rotary_heads");
+  if (layout != KB_ROPE_PAIRS && layout != KB_ROPE_HALVES) return bad("layout must be KB_ROPE_PAIRS or KB_ROPE_HALVES");
+  if (x_token < 0 || x_head < 0 || out_token < 0 || out_head < 0 || (slots && out_rows < 0))
+    return bad("strides and out_rows must not be negative");
+  if (tokens == 0) return KB_OK;
+  if (!x || !out || !positions || !freqs) return bad("null pointer");
+  const int es = dtype == KB_DT_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(x) % es || reinterpret_cast<uintptr_t>(out) % es)
+    return bad("x and out must be aligned to their elements");
+  // out's rows and heads must be disjoint, whichever of the two is outer
+  const int64_t rows = slots ? out_rows : tokens, most = int64_t(1) << 40;
+  if (x_token > most || x_head > most || out_token > most || out_head > most) return bad("strides above 2^40 elements");
+  const int64_t head_span = (heads - 1) * out_head + head_dim;
+  const bool token_outer = (heads == 1 || out_head >= head_dim) && (rows <= 1 || out_token >= head_span);
+  const bool head_outer = (rows <= 1 || out_token >= head_dim) &&
+                          (heads == 1 || (rows <= (int64_t(1) << 22) && out_head >= (rows - 1) * out_token + head_dim));
+  if (!token_outer && !head_outer) return bad("out's rows and heads must not overlap");
+  if (x == out && (slots || x_token != out_token || x_head != out_head))
+    return bad("in place needs equal strides and no slots");
+  RopeArgs a;
+  a.x = x, a.positions = positions, a.freqs = freqs, a.slots = slots, a.out = out;
+  a.x_token = x_token, a.x_head = x_head, a.out_token = out_token, a.out_head = out_head, a.out_rows = out_rows;
+  a.tokens = tokens, a.head_dim = head_dim, a.pairs = pairs, a.rotary_heads = rotary_heads;
+  a.freq_head_stride = freq_heads == 1 ? 0 : pairs * axes;
+  a.f16 = dtype == KB_DT_F16;
+  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  // Four elements per access need 8- or 16-byte addresses and whole groups;
+  // anything else takes the kernel of single elements.
+  const uintptr_t align = 4 * es;
+  const bool vec = head_dim % 8 == 0 && x_token % 4 == 0 && x_head % 4 == 0 && out_token % 4 == 0 &&
+                   out_head % 4 == 0 && reinterpret_cast<uintptr_t>(x) % align == 0 &&
+                   reinterpret_cast<uintptr_t>(out) % align == 0 && (layout == KB_ROPE_PAIRS || pairs % 4 == 0);
+  const bool halves = layout == KB_ROPE_HALVES;
+  if (es == 2) {
+    if (vec) return halves ? launch<uint16_t, 4, true>(a, heads, axes, s) : launch<uint16_t, 4, false>(a, heads, axes, s);
+    return halves ? launch<uint16_t, 1, true>(a, heads, axes, s) : launch<uint16_t, 1, false>(a, heads, axes, s);
+  }
+  if (vec) return halves ? launch<float, 4, true>(a, heads, axes, s) : launch<float, 4, false>(a, heads, axes, s);
+  return halves ? launch<float, 1, true>(a, heads, axes, s) : launch<float, 1, false>(a, heads, axes, s);
+}
