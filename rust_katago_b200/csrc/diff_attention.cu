@@ -88,6 +88,78 @@ __global__ void __launch_bounds__(128) diff_simple_kernel(const DiffArgs a) {
   }
 }
 
+// Joins the parts of a row whose keys were split over blocks: one warp per
+// row, the parts in order, each weighted by 2^(its maximum - the row's).
+template <int D>
+__global__ void __launch_bounds__(128) diff_combine_kernel(const DiffArgs a, int splits) {
+  constexpr int kE = 2 * D / 32;
+  const int lane = threadIdx.x & 31;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  if (row >= static_cast<int64_t>(a.d.batch) * a.d.q_len * a.d.heads) return;
+  const int h = static_cast<int>(row % a.d.heads);
+  const int64_t bi = row / a.d.heads;
+  float acc[2][kE], mm[2], ll[2];
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    const float2* ml = a.part_ml + row * splits * 2 + m;
+    float top = -INFINITY;
+    for (int s = lane; s < splits; s += 32) top = fmaxf(top, ml[2 * s].x);
+#pragma unroll
+    for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    mm[m] = top, ll[m] = 0.0f;
+#pragma unroll
+    for (int e = 0; e < kE; ++e) acc[m][e] = 0.0f;
+    const float* part = a.part_o + (row * splits * 2 + m) * (2 * D) + lane * kE;
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) {
+      const float2 v = ml[2 * s];
+      const float f = v.x == -INFINITY ? 0.0f : exp2f(v.x - top);
+      ll[m] += f * v.y;
+      float o[kE];
+      if constexpr (kE == 4) *reinterpret_cast<float4*>(o) = *reinterpret_cast<const float4*>(part + s * (4 * D));
+      else *reinterpret_cast<float2*>(o) = *reinterpret_cast<const float2*>(part + s * (4 * D));
+#pragma unroll
+      for (int e = 0; e < kE; ++e) acc[m][e] = fmaf(f, o[e], acc[m][e]);
+    }
+  }
+  finish_row<kE>(a, static_cast<int>(bi / a.d.q_len), static_cast<int>(bi % a.d.q_len), h, lane, acc, mm, ll);
+}
+
+// How a call runs: rows (queries x heads of a group) up to kFewRows by the
+// kernel for few queries, with its keys split over blocks.
+struct Plan {
+  bool few = false;
+  int splits = 1;
+};
+
+constexpr int kFewRows = 16;
+constexpr int kFewKeys = 128;  // keys per block of four warps, at least
+
+Plan make_plan(const kb_diff_attention_desc& d) {
+  Plan p;
+  const int64_t rows = static_cast<int64_t>(d.q_len) * (d.heads / d.kv_heads);
+  p.few = rows <= kFewRows;
+  if (p.few) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    int64_t keys = d.kv_len;
+    if (d.window && keys > static_cast<int64_t>(d.window) + d.q_len) keys = static_cast<int64_t>(d.window) + d.q_len;
+    const int64_t units = static_cast<int64_t>(d.batch) * d.kv_heads;
+    const int64_t want = (3 * static_cast<int64_t>(num_sms(dev)) + units - 1) / units;
+    const int64_t most = (keys + kFewKeys - 1) / kFewKeys;
+    const int64_t s = want < most ? want : most;
+    p.splits = static_cast<int>(s < 1 ? 1 : s > 1024 ? 1024 : s);
+  }
+  return p;
+}
+
+size_t partial_bytes(const kb_diff_attention_desc& d, int splits, size_t* o_offset) {
+  const size_t parts = static_cast<size_t>(d.batch) * d.q_len * d.heads * splits * 2;
+  const size_t at = (parts * sizeof(float2) + 127) / 128 * 128;
+  if (o_offset) *o_offset = at;
+  return at + parts * 2 * d.head_dim * sizeof(float);
+}
+
 int bad(const char* what) {
   set_error(std::string("kb_diff_attention: ") + what);
   return KB_E_INVALID;
@@ -119,6 +191,21 @@ int check_desc(const kb_diff_attention_desc* desc) {
 }
 
 }  // namespace
+
+int diff_combine_launch(const DiffArgs& a, int splits, cudaStream_t s) {
+  const int64_t rows = static_cast<int64_t>(a.d.batch) * a.d.q_len * a.d.heads;
+  const unsigned grid = static_cast<unsigned>((rows + 3) / 4);
+  if (a.d.head_dim == 64) diff_combine_kernel<64><<<grid, 128, 0, s>>>(a, splits);
+  else diff_combine_kernel<32><<<grid, 128, 0, s>>>(a, splits);
+  return check_cuda(cudaGetLastError(), "differential attention join launch");
+}
+
+// Allow `kernel` to use `bytes` of dynamic shared memory on the current device.
+int smem_opt_in(const void* kernel, int bytes) {
+  return check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes),
+                    "differential attention smem attribute");
+}
+
 }  // namespace kb
 
 extern "C" int kb_diff_attention_workspace(const kb_diff_attention_desc* desc, size_t* bytes) {
@@ -127,6 +214,9 @@ extern "C" int kb_diff_attention_workspace(const kb_diff_attention_desc* desc, s
   if (rc) return rc;
   if (!bytes) return bad("null bytes");
   *bytes = 0;
+  if (desc->batch == 0 || desc->q_len == 0) return KB_OK;
+  const Plan p = make_plan(*desc);
+  if (p.splits > 1) *bytes = partial_bytes(*desc, p.splits, nullptr);
   return KB_OK;
 }
 
@@ -151,8 +241,19 @@ extern "C" int kb_diff_attention(const kb_diff_attention_desc* desc, const uint1
     set_error("kb_diff_attention: workspace of " + std::to_string(need) + " bytes needed");
     return KB_E_INVALID;
   }
-  const DiffArgs a = make_diff_args(d, q, k, v, lambda, gamma, kv_lens, key_mask, out);
+  DiffArgs a = make_diff_args(d, q, k, v, lambda, gamma, kv_lens, key_mask, out);
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const Plan p = make_plan(d);
+  if (p.splits > 1) {
+    size_t at = 0;
+    partial_bytes(d, p.splits, &at);
+    a.part_ml = static_cast<float2*>(workspace);
+    a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + at);
+  }
+  if (p.few) {
+    const int rc2 = diff_decode_launch(a, p.splits, s);
+    return rc2 || p.splits == 1 ? rc2 : diff_combine_launch(a, p.splits, s);
+  }
   const int64_t jobs = static_cast<int64_t>(d.batch) * d.heads * d.q_len;
   if ((jobs + 3) / 4 > 0x7fffffff) return bad("too many queries");
   const unsigned grid = static_cast<unsigned>((jobs + 3) / 4);

@@ -1,0 +1,360 @@
+// Differential attention of few queries over many keys: single tokens, and
+// short pieces whose queries and grouped heads fill at most a few tiles.
+//
+// Every key and value has to be read once, 8 D bytes per key and key/value
+// head, for 12 D flop per query: HBM bounds it, so what counts is bytes in
+// flight and no work between them.
+//
+// A warp takes 16 keys at a time with mma.sync in transposed form: S^T = K Q^T
+// (16 keys x 8 rows) and O^T = V^T P^T (16 value dims x 8 rows), so a tile is 8
+// rows wide (rows: queries x heads of the group) instead of the 16 that queries
+// as the M side would pad to.  mma.sync and not tcgen05: a tcgen05 tile is 128
+// rows of which one is used, and its operands must pass through shared memory;
+// here each thread's fragments are 16-byte pieces of the K and V rows in
+// global memory, taken straight into registers.  That needs no order of dims
+// in memory: the contraction over head dims uses the same permutation for Q,
+// and value dims come out permuted, eight neighbours per thread.  The loads of
+// the next K go out while the softmax and the value product of the current 16
+// keys run, those of the next V before the next score product.
+// P is rounded to the 16-bit type for the value product; sums are taken of the
+// unrounded P in fp32.  The running maximum moves only when a score exceeds it
+// by 2^8, so most steps skip the reduction over keys and the rescaling.
+//
+// Keys are split over blocks (partial results through the workspace, joined by
+// diff_combine) and within a block over its warps (joined in shared memory), in
+// a fixed order: results do not depend on timing.
+#include <math.h>
+#include <stdint.h>
+
+#include "kb_diff.cuh"
+#include "kb_internal.h"
+#include "kb_numeric.cuh"
+
+namespace kb {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr float kLazy = 8.0f;  // log2 of how far a score may exceed the running maximum
+
+template <bool F16>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (F16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Transpose an 8 x 8 matrix of 16-bit values held as two per thread.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+__device__ __forceinline__ uint4 load16(const uint16_t* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+// NR: 8-row tiles per warp.
+template <int D, int NR, bool F16>
+__global__ void __launch_bounds__(32 * kWarps, NR == 1 ? 3 : 2) diff_decode_kernel(const DiffArgs a, int row_tiles) {
+  constexpr int kCh = D / 32;   // 16-byte pieces per thread of a K row, and of half a V row
+  constexpr int kKs = D / 16;   // steps of the score product
+  constexpr int kMt = D / 8;    // 16-dim tiles of the value product
+  constexpr int kRows = 8 * NR, kDv = 2 * D;
+  extern __shared__ float sm[];  // [warp][row][map]: kDv sums; then {m, l}
+  const kb_diff_attention_desc& d = a.d;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int share = d.heads / d.kv_heads;
+  const int hk = blockIdx.y / row_tiles, r0 = (blockIdx.y % row_tiles) * kRows;
+  const int b = blockIdx.z, split = blockIdx.x, splits = gridDim.x;
+  const int rows = min(kRows, d.q_len * share - r0);  // valid rows of this tile
+
+  // Keys of the tile, of this split, and of each row held by this thread.
+  const int n = key_count(a, b);
+  int first, last;
+  key_range_n(d, n, r0 / share, (r0 + rows - 1) / share, first, last);
+  const int steps = (max(0, last - first) + 15) / 16;
+  const int per = (steps + splits - 1) / splits * 16;
+  const int s0 = min(last, first + split * per), s1 = min(last, s0 + per);
+  int common_lo = 0, common_hi = n;  // keys that every row sees
+  if (d.causal) {
+    common_hi = min(n, n - d.q_len + r0 / share + 1);
+    if (d.window) common_lo = max(0, n - d.q_len + (r0 + rows - 1) / share + 1 - d.window);
+  }
+  int lo[NR][2], hi[NR][2];
+#pragma unroll
+  for (int t = 0; t < NR; ++t)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int r = r0 + 8 * t + 2 * c + u;
+      key_range_n(d, n, r / share, r / share, lo[t][u], hi[t][u]);
+    }
+  const uint8_t* mask = a.key_mask ? a.key_mask + b * d.mask_batch : nullptr;
+
+  // Q as the B operand: row g of each 8-row tile, dims permuted as K's are.
+  uint32_t qf[2][NR][kKs][2];
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int t = 0; t < NR; ++t) {
+      const int r = r0 + 8 * t + g;
+      const bool ok = 8 * t + g < rows;
+#pragma unroll
+      for (int x = 0; x < kCh; ++x) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (ok) v = load16(a.q + b * d.q_batch + (r / share) * d.q_token + (hk * share + r % share) * d.q_head + m * d.q_map + x * 32 + c * 8);
+        qf[m][t][2 * x][0] = v.x, qf[m][t][2 * x][1] = v.y, qf[m][t][2 * x + 1][0] = v.z, qf[m][t][2 * x + 1][1] = v.w;
+      }
+    }
+
+  float mx[2][NR][2], l[2][NR][2], o[2][NR][kMt][4];
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int t = 0; t < NR; ++t) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) mx[m][t][u] = -INFINITY, l[m][t][u] = 0.0f;
+#pragma unroll
+      for (int x = 0; x < kMt; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[m][t][x][e] = 0.0f;
+    }
+
+  uint4 kf[2][2][kCh], vv[4][kCh];
+  const uint16_t* kbase = a.k + b * d.k_batch + hk * d.k_head + c * 8;
+  const uint16_t* vbase = a.v + b * d.v_batch + hk * d.v_head + g * 8;
+  auto load_k = [&](int j) {
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      const int key = j + g + 8 * y;
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int x = 0; x < kCh; ++x)
+          kf[m][y][x] = key < s1 ? load16(kbase + key * d.k_token + m * d.k_map + x * 32) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  // V: keys 2c, 2c + 1, 2c + 8, 2c + 9, dims 8g.. (and 64 + 8g.. for D = 64).
+  auto load_v = [&](int j) {
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const int key = j + 2 * c + (y & 1) + 8 * (y >> 1);
+#pragma unroll
+      for (int x = 0; x < kCh; ++x)
+        vv[y][x] = key < s1 ? load16(vbase + key * d.v_token + x * 64) : make_uint4(0, 0, 0, 0);
+    }
+  };
+
+  int j = s0 + 16 * warp;
+  if (j < s1) {
+    load_k(j);
+    load_v(j);
+  }
+  for (; j < s1; j += 16 * kWarps) {
+    float s[2][NR][4];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int t = 0; t < NR; ++t) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[m][t][e] = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < kKs; ++ks) {
+          const uint4 &k0 = kf[m][0][ks / 2], &k1 = kf[m][1][ks / 2];
+          const uint32_t af[4] = {word(k0, 2 * (ks & 1)), word(k1, 2 * (ks & 1)), word(k0, 2 * (ks & 1) + 1),
+                                  word(k1, 2 * (ks & 1) + 1)};
+          mma16816<F16>(s[m][t], af, qf[m][t][ks][0], qf[m][t][ks][1]);
+        }
+      }
+    if (j + 16 * kWarps < s1) load_k(j + 16 * kWarps);
+
+    // Scores to log2 units, hidden ones to -inf; values of hidden keys to zero.
+    const bool inside = j >= common_lo && j + 16 <= common_hi && mask == nullptr;
+    bool see0 = true, see1 = true;
+    if (!inside) {
+      see0 = j + g < s1 && (mask == nullptr || mask[j + g]);
+      see1 = j + g + 8 < s1 && (mask == nullptr || mask[j + g + 8]);
+      if (mask) {
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const int key = j + 2 * c + (y & 1) + 8 * (y >> 1);
+          if (key < s1 && !mask[key])
+#pragma unroll
+            for (int x = 0; x < kCh; ++x) vv[y][x] = make_uint4(0, 0, 0, 0);
+        }
+      }
+    }
+    bool grow = false;
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int t = 0; t < NR; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float x = s[m][t][e] * a.scale_log2;
+          if (!inside) {
+            const int key = j + g + 8 * (e >> 1);
+            const bool see = (e >> 1 ? see1 : see0) && key >= lo[t][e & 1] && key < hi[t][e & 1];
+            x = see ? x : -INFINITY;
+          }
+          s[m][t][e] = x;
+          grow |= x > mx[m][t][e & 1] + kLazy || (mx[m][t][e & 1] == -INFINITY && x > -INFINITY);
+        }
+    if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int t = 0; t < NR; ++t)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            float v = fmaxf(mx[m][t][u], fmaxf(s[m][t][u], s[m][t][u + 2]));
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, x));
+            const float f = mx[m][t][u] == -INFINITY ? 1.0f : exp2_fast(mx[m][t][u] - v);  // sums are 0 before the first key
+            mx[m][t][u] = v;
+            l[m][t][u] *= f;
+#pragma unroll
+            for (int x = 0; x < kMt; ++x) o[m][t][x][u] *= f, o[m][t][x][u + 2] *= f;
+          }
+    }
+    uint32_t pf[2][NR][2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int t = 0; t < NR; ++t) {
+        float p[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float base = mx[m][t][e & 1];
+          p[e] = exp2_fast(s[m][t][e] - (base == -INFINITY ? 0.0f : base));
+          l[m][t][e & 1] += p[e];
+        }
+        pf[m][t][0] = transpose8(pack16x2(make_float2(p[0], p[1]), F16));
+        pf[m][t][1] = transpose8(pack16x2(make_float2(p[2], p[3]), F16));
+      }
+    // O^T += V^T P^T: tile x holds dims {lower: a0, a2; upper: a1, a3} of every g
+#pragma unroll
+    for (int x = 0; x < kMt; ++x) {
+      uint32_t af[4];
+      if constexpr (D == 64) {
+        const int w = (x & 7) >> 1;
+        const uint32_t sel = x & 1 ? 0x7632 : 0x5410;
+        af[0] = __byte_perm(word(vv[0][0], w), word(vv[1][0], w), sel);
+        af[1] = __byte_perm(word(vv[0][1], w), word(vv[1][1], w), sel);
+        af[2] = __byte_perm(word(vv[2][0], w), word(vv[3][0], w), sel);
+        af[3] = __byte_perm(word(vv[2][1], w), word(vv[3][1], w), sel);
+      } else {  // 64 dims: tile x holds dims 8g + 2x (lower) and 8g + 2x + 1 (upper)
+        af[0] = __byte_perm(word(vv[0][0], x), word(vv[1][0], x), 0x5410);
+        af[1] = __byte_perm(word(vv[0][0], x), word(vv[1][0], x), 0x7632);
+        af[2] = __byte_perm(word(vv[2][0], x), word(vv[3][0], x), 0x5410);
+        af[3] = __byte_perm(word(vv[2][0], x), word(vv[3][0], x), 0x7632);
+      }
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int t = 0; t < NR; ++t) mma16816<F16>(o[m][t][x], af, pf[m][t][0], pf[m][t][1]);
+    }
+    if (j + 16 * kWarps < s1) load_v(j + 16 * kWarps);
+  }
+
+  // Sums over the keys of the warp's lanes, then the warps' parts to shared memory.
+  float2* ml = reinterpret_cast<float2*>(sm + kWarps * kRows * 2 * kDv);
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int t = 0; t < NR; ++t)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float v = l[m][t][u];
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) v += __shfl_xor_sync(0xffffffffu, v, x);
+        const int row = 8 * t + 2 * c + u;
+        float* dst = sm + ((warp * kRows + row) * 2 + m) * kDv;
+        if (g == 0) ml[(warp * kRows + row) * 2 + m] = make_float2(mx[m][t][u], v);
+#pragma unroll
+        for (int x = 0; x < kMt; ++x) {
+          if constexpr (D == 64) {
+            dst[8 * g + x] = o[m][t][x][u];
+            dst[64 + 8 * g + x] = o[m][t][x][u + 2];
+          } else {
+            dst[8 * g + 2 * x] = o[m][t][x][u];
+            dst[8 * g + 2 * x + 1] = o[m][t][x][u + 2];
+          }
+        }
+      }
+  __syncthreads();
+  // One warp per row joins the warps' parts; lanes hold kDv / 32 dims.
+  constexpr int kE = kDv / 32;
+  for (int row = warp; row < rows; row += kWarps) {
+    const int r = r0 + row, i = r / share, h = hk * share + r % share;
+    float acc[2][kE], mm[2], ll[2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      mm[m] = -INFINITY, ll[m] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) mm[m] = fmaxf(mm[m], ml[(w * kRows + row) * 2 + m].x);
+#pragma unroll
+      for (int e = 0; e < kE; ++e) acc[m][e] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float2 v = ml[(w * kRows + row) * 2 + m];
+        const float f = v.x == -INFINITY ? 0.0f : exp2_fast(v.x - mm[m]);
+        ll[m] += f * v.y;
+        const float* src = sm + ((w * kRows + row) * 2 + m) * kDv + lane * kE;
+#pragma unroll
+        for (int e = 0; e < kE; ++e) acc[m][e] = fmaf(f, src[e], acc[m][e]);
+      }
+    }
+    if (splits == 1) {
+      finish_row<kE>(a, b, i, h, lane, acc, mm, ll);
+    } else {
+      write_partial<kE>(a, splits, split, b, i, h, lane, acc, mm, ll);
+    }
+  }
+}
+
+template <int D, int NR, bool F16>
+int launch(const DiffArgs& a, int splits, cudaStream_t s) {
+  constexpr int kBytes = kWarps * 8 * NR * 2 * (2 * D * 4 + 8);
+  const int rows = a.d.q_len * (a.d.heads / a.d.kv_heads);
+  const int row_tiles = (rows + 8 * NR - 1) / (8 * NR);
+  auto kern = diff_decode_kernel<D, NR, F16>;
+  if constexpr (kBytes > 48 * 1024) {
+    const int rc = smem_opt_in(reinterpret_cast<const void*>(kern), kBytes);
+    if (rc) return rc;
+  }
+  kern<<<dim3(splits, a.d.kv_heads * row_tiles, a.d.batch), 32 * kWarps, kBytes, s>>>(a, row_tiles);
+  return check_cuda(cudaGetLastError(), "differential attention (few queries) launch");
+}
+
+}  // namespace
+
+int diff_decode_launch(const DiffArgs& a, int splits, cudaStream_t s) {
+  const bool f16 = a.d.dtype == KB_DT_F16;
+  const bool wide = a.d.q_len * (a.d.heads / a.d.kv_heads) > 8;
+  if (a.d.head_dim == 64) {
+    if (wide) return f16 ? launch<64, 2, true>(a, splits, s) : launch<64, 2, false>(a, splits, s);
+    return f16 ? launch<64, 1, true>(a, splits, s) : launch<64, 1, false>(a, splits, s);
+  }
+  if (wide) return f16 ? launch<32, 2, true>(a, splits, s) : launch<32, 2, false>(a, splits, s);
+  return f16 ? launch<32, 1, true>(a, splits, s) : launch<32, 1, false>(a, splits, s);
+}
+
+}  // namespace kb

@@ -2,9 +2,11 @@
 // range of keys that a group of queries sees.
 #pragma once
 
+#include <math.h>
 #include <stdint.h>
 
 #include "../../include/katab200.h"
+#include "kb_numeric.cuh"
 
 namespace kb {
 
@@ -16,13 +18,18 @@ struct DiffArgs {
   const uint8_t* key_mask;
   uint16_t* out;
   float scale_log2;  // scale * log2(e): the kernels' exponentials are powers of two
+  // Partial results of keys split over blocks (workspace), per row (b, i, h),
+  // split and map: {running maximum (log2 units), sum}, and 2 head_dim value sums.
+  float2* part_ml;
+  float* part_o;
 };
 
 // Strides of dimensions of extent 1 are set to 0, so no address depends on them.
 inline DiffArgs make_diff_args(const kb_diff_attention_desc& desc, const uint16_t* q, const uint16_t* k,
                                const uint16_t* v, const float* lambda, const float* gamma, const int32_t* kv_lens,
                                const uint8_t* key_mask, uint16_t* out) {
-  DiffArgs a{desc, q, k, v, lambda, gamma, kv_lens, key_mask, out, desc.scale * 1.4426950408889634f};
+  DiffArgs a{desc, q, k, v, lambda, gamma, kv_lens, key_mask, out, desc.scale * 1.4426950408889634f,
+             nullptr, nullptr};
   kb_diff_attention_desc& d = a.d;
   if (d.batch == 1) d.q_batch = d.k_batch = d.v_batch = d.out_batch = d.mask_batch = 0;
   if (d.q_len == 1) d.q_token = d.out_token = 0;
@@ -52,5 +59,56 @@ __device__ __forceinline__ void key_range_n(const kb_diff_attention_desc& d, int
 __device__ __forceinline__ void key_range(const DiffArgs& a, int b, int i0, int i1, int& first, int& last) {
   key_range_n(a.d, key_count(a, b), i0, i1, first, last);
 }
+
+__device__ __forceinline__ int64_t row_index(const DiffArgs& a, int b, int i, int h) {
+  return (static_cast<int64_t>(b) * a.d.q_len + i) * a.d.heads + h;
+}
+
+// A row's result from both maps' sums `acc` (kE dims per lane, dims lane kE..),
+// maxima and weights: the weighted difference, its norm, one rounding.  Whole warps.
+template <int kE>
+__device__ __forceinline__ void finish_row(const DiffArgs& a, int b, int i, int h, int lane, const float (&acc)[2][kE],
+                                           const float (&mm)[2], const float (&ll)[2]) {
+  const float w0 = mm[0] == -INFINITY ? 0.0f : 1.0f / ll[0];
+  const float w1 = mm[1] == -INFINITY ? 0.0f : a.lambda[h] / ll[1];
+  float r[kE], ss = 0.0f;
+#pragma unroll
+  for (int e = 0; e < kE; ++e) {
+    r[e] = acc[0][e] * w0 - acc[1][e] * w1;
+    ss = fmaf(r[e], r[e], ss);
+  }
+  float f = a.d.out_scale;
+  if (a.gamma) {
+#pragma unroll
+    for (int x = 16; x; x >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, x);
+    f *= 1.0f / sqrtf(ss / (32 * kE) + a.d.eps);
+  }
+  uint16_t* out = a.out + b * a.d.out_batch + i * a.d.out_token + h * a.d.out_head + lane * kE;
+  uint32_t w[kE / 2];
+#pragma unroll
+  for (int e = 0; e < kE; e += 2) {
+    const float g0 = a.gamma ? a.gamma[lane * kE + e] : 1.0f, g1 = a.gamma ? a.gamma[lane * kE + e + 1] : 1.0f;
+    w[e / 2] = pack16x2(make_float2(r[e] * f * g0, r[e + 1] * f * g1), a.d.dtype == KB_DT_F16);
+  }
+  if constexpr (kE == 4) *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
+  else *reinterpret_cast<uint32_t*>(out) = w[0];
+}
+
+template <int kE>
+__device__ __forceinline__ void write_partial(const DiffArgs& a, int splits, int split, int b, int i, int h, int lane,
+                                              const float (&acc)[2][kE], const float (&mm)[2], const float (&ll)[2]) {
+  const int64_t at = (row_index(a, b, i, h) * splits + split) * 2;
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    if (lane == 0) a.part_ml[at + m] = make_float2(mm[m], ll[m]);
+    float* dst = a.part_o + (at + m) * (32 * kE) + lane * kE;
+    if constexpr (kE == 4) *reinterpret_cast<float4*>(dst) = make_float4(acc[m][0], acc[m][1], acc[m][2], acc[m][3]);
+    else *reinterpret_cast<float2*>(dst) = make_float2(acc[m][0], acc[m][1]);
+  }
+}
+
+int diff_decode_launch(const DiffArgs& a, int splits, cudaStream_t s);
+int diff_combine_launch(const DiffArgs& a, int splits, cudaStream_t s);
+int smem_opt_in(const void* kernel, int bytes);
 
 }  // namespace kb
