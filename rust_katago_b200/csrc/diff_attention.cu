@@ -12,82 +12,6 @@
 namespace kb {
 namespace {
 
-// One warp per (batch, head, query); lanes take one key each for the two dot
-// products and the running maxima and sums, then 2D / 32 dims each of the two
-// value sums.
-template <int D>
-__global__ void __launch_bounds__(128) diff_simple_kernel(const DiffArgs a) {
-  constexpr int kDims = 2 * D / 32;
-  __shared__ float qs[4][2 * D];
-  const kb_diff_attention_desc& d = a.d;
-  const bool f16 = d.dtype == KB_DT_F16;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t job = static_cast<int64_t>(blockIdx.x) * 4 + warp;
-  if (job >= static_cast<int64_t>(d.batch) * d.heads * d.q_len) return;
-  const int i = static_cast<int>(job % d.q_len);
-  const int h = static_cast<int>(job / d.q_len % d.heads);
-  const int b = static_cast<int>(job / d.q_len / d.heads);
-  const int hk = h / (d.heads / d.kv_heads);
-  for (int c = lane; c < 2 * D; c += 32)
-    qs[warp][c] = from16(a.q[b * d.q_batch + i * d.q_token + h * d.q_head + (c / D) * d.q_map + c % D], f16);
-  __syncwarp();
-  int first, last;
-  key_range(a, b, i, i, first, last);
-  const uint16_t* k0 = a.k + b * d.k_batch + hk * d.k_head;
-  const uint16_t* v0 = a.v + b * d.v_batch + hk * d.v_head;
-  const uint8_t* mask = a.key_mask ? a.key_mask + b * d.mask_batch : nullptr;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[2][kDims] = {};
-  for (int j0 = first; j0 < last; j0 += 32) {
-    const int j = j0 + lane;
-    const bool see = j < last && (!mask || mask[j]);
-    float p[2];
-    for (int t = 0; t < 2; ++t) {
-      float s = -INFINITY;
-      if (see) {
-        const uint16_t* kr = k0 + j * d.k_token + t * d.k_map;
-        s = 0.0f;
-        for (int c = 0; c < D; ++c) s = fmaf(qs[warp][t * D + c], from16(kr[c], f16), s);
-        s *= a.scale_log2;
-      }
-      float mt = s;
-      for (int x = 16; x; x >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, x));
-      const float mn = fmaxf(m[t], mt);
-      const float base = mn == -INFINITY ? 0.0f : mn;
-      const float f = exp2f(m[t] - base);
-      p[t] = exp2f(s - base);
-      m[t] = mn;
-      l[t] = l[t] * f + p[t];
-      for (int c = 0; c < kDims; ++c) o[t][c] *= f;
-    }
-    for (int u = 0; u < 32; ++u) {
-      const float p0 = __shfl_sync(0xffffffffu, p[0], u), p1 = __shfl_sync(0xffffffffu, p[1], u);
-      const bool use = __shfl_sync(0xffffffffu, static_cast<int>(see), u);
-      if (!use) continue;
-      for (int c = 0; c < kDims; ++c) {
-        const float v = from16(v0[(j0 + u) * d.v_token + c * 32 + lane], f16);
-        o[0][c] = fmaf(p0, v, o[0][c]);
-        o[1][c] = fmaf(p1, v, o[1][c]);
-      }
-    }
-  }
-  for (int t = 0; t < 2; ++t)
-    for (int x = 16; x; x >>= 1) l[t] += __shfl_xor_sync(0xffffffffu, l[t], x);
-  const float w0 = m[0] == -INFINITY ? 0.0f : 1.0f / l[0];
-  const float w1 = m[1] == -INFINITY ? 0.0f : a.lambda[h] / l[1];
-  float ss = 0.0f, r[kDims];
-  for (int c = 0; c < kDims; ++c) {
-    r[c] = o[0][c] * w0 - o[1][c] * w1;
-    ss = fmaf(r[c], r[c], ss);
-  }
-  for (int x = 16; x; x >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, x);
-  const float rstd = a.gamma ? 1.0f / sqrtf(ss / (2 * D) + d.eps) : 1.0f;
-  uint16_t* out = a.out + b * d.out_batch + i * d.out_token + h * d.out_head;
-  for (int c = 0; c < kDims; ++c) {
-    const float g = a.gamma ? a.gamma[c * 32 + lane] : 1.0f;
-    out[c * 32 + lane] = bits16(r[c] * rstd * g * d.out_scale, f16);
-  }
-}
-
 // Joins the parts of a row whose keys were split over blocks: one warp per
 // row, the parts in order, each weighted by 2^(its maximum - the row's).
 template <int D>
@@ -113,7 +37,10 @@ __global__ void __launch_bounds__(128) diff_combine_kernel(const DiffArgs a, int
 #pragma unroll 4
     for (int s = 0; s < splits; ++s) {
       const float2 v = ml[2 * s];
-      const float f = v.x == -INFINITY ? 0.0f : exp2f(v.x - top);
+      // A part that saw no key: its value sums may not have been written.  (A
+      // NaN sum without a maximum is a row of NaN scores and has to go on.)
+      if (v.x == -INFINITY && v.y == 0.0f) continue;
+      const float f = exp2f(v.x - top);
       ll[m] += f * v.y;
       float o[kE];
       if constexpr (kE == 4) *reinterpret_cast<float4*>(o) = *reinterpret_cast<const float4*>(part + s * (4 * D));
@@ -122,7 +49,7 @@ __global__ void __launch_bounds__(128) diff_combine_kernel(const DiffArgs a, int
       for (int e = 0; e < kE; ++e) acc[m][e] = fmaf(f, o[e], acc[m][e]);
     }
   }
-  finish_row<kE>(a, static_cast<int>(bi / a.d.q_len), static_cast<int>(bi % a.d.q_len), h, lane, acc, mm, ll);
+  finish_row<kE>(a, static_cast<int>(bi / a.d.q_len), static_cast<int>(bi % a.d.q_len), h, lane, acc, ll);
 }
 
 // How a call runs: rows (queries x heads of a group) up to kFewRows by the
@@ -134,21 +61,29 @@ struct Plan {
 
 constexpr int kFewRows = 16;
 constexpr int kFewKeys = 128;  // keys per block of four warps, at least
+constexpr int kTileKeys = 128;
+constexpr int kTilesPerSplit = 4;
 
 Plan make_plan(const kb_diff_attention_desc& d) {
   Plan p;
   const int64_t rows = static_cast<int64_t>(d.q_len) * (d.heads / d.kv_heads);
-  p.few = rows <= kFewRows;
+  p.few = rows <= kFewRows || d.kv_len == 0;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  int64_t keys = d.kv_len;
+  if (d.window && keys > static_cast<int64_t>(d.window) + d.q_len) keys = static_cast<int64_t>(d.window) + d.q_len;
   if (p.few) {
-    int dev = 0;
-    cudaGetDevice(&dev);
-    int64_t keys = d.kv_len;
-    if (d.window && keys > static_cast<int64_t>(d.window) + d.q_len) keys = static_cast<int64_t>(d.window) + d.q_len;
     const int64_t units = static_cast<int64_t>(d.batch) * d.kv_heads;
     const int64_t want = (3 * static_cast<int64_t>(num_sms(dev)) + units - 1) / units;
     const int64_t most = (keys + kFewKeys - 1) / kFewKeys;
     const int64_t s = want < most ? want : most;
     p.splits = static_cast<int>(s < 1 ? 1 : s > 1024 ? 1024 : s);
+  } else {
+    const int64_t tiles = (keys + kTileKeys - 1) / kTileKeys;
+    const int64_t units = static_cast<int64_t>(d.batch) * d.heads * ((d.q_len + 127) / 128);
+    const int64_t want = num_sms(dev) / units, most = tiles / kTilesPerSplit;
+    const int64_t s = want < most ? want : most;
+    p.splits = static_cast<int>(s < 1 ? 1 : s > 64 ? 64 : s);
   }
   return p;
 }
@@ -175,7 +110,8 @@ int check_desc(const kb_diff_attention_desc* desc) {
     return bad("at most 65535 sequences, 2^26 queries, 2^30 keys and 1024 heads");
   if (d.heads < 1 || d.kv_heads < 1 || d.heads % d.kv_heads) return bad("heads must be a multiple of kv_heads");
   if (d.window < 0 || (d.window > 0 && !d.causal)) return bad("a window must be positive and causal");
-  if (!isfinite(d.scale) || !isfinite(d.out_scale) || !(d.eps >= 0.0f)) return bad("scale, out_scale or eps");
+  if (!(d.scale > 0.0f) || !isfinite(d.scale) || !isfinite(d.out_scale) || !(d.eps >= 0.0f))
+    return bad("a positive scale, a finite out_scale and eps >= 0 expected");
   const int64_t most = int64_t(1) << 38;
   auto ok = [&](int64_t stride, int64_t extent) { return extent <= 1 || (stride >= 0 && stride < most && stride % 8 == 0); };
   if (!ok(d.q_batch, d.batch) || !ok(d.q_token, d.q_len) || !ok(d.q_head, d.heads) || !ok(d.q_map, 2) ||
@@ -183,6 +119,8 @@ int check_desc(const kb_diff_attention_desc* desc) {
       !ok(d.v_batch, d.batch) || !ok(d.v_token, d.kv_len) || !ok(d.v_head, d.kv_heads) ||
       !ok(d.out_batch, d.batch) || !ok(d.out_token, d.q_len) || !ok(d.out_head, d.heads))
     return bad("strides must be multiples of 8 elements, not negative and below 2^38");
+  if ((d.q_len > 1 && d.q_token == 0) || (d.kv_len > 1 && (d.k_token == 0 || d.v_token == 0)))
+    return bad("tokens cannot be broadcast");
   auto apart = [&](int64_t stride, int64_t extent) { return extent <= 1 || stride >= 2 * d.head_dim; };
   if (!apart(d.out_batch, d.batch) || !apart(d.out_token, d.q_len) || !apart(d.out_head, d.heads))
     return bad("out's rows must not overlap");
@@ -225,7 +163,6 @@ extern "C" int kb_diff_attention(const kb_diff_attention_desc* desc, const uint1
                                  const uint8_t* key_mask, uint16_t* out, void* workspace, size_t workspace_bytes,
                                  uint32_t* status, uintptr_t stream) {
   using namespace kb;
-  (void)status;
   const int rc = check_desc(desc);
   if (rc) return rc;
   const kb_diff_attention_desc& d = *desc;
@@ -250,16 +187,8 @@ extern "C" int kb_diff_attention(const kb_diff_attention_desc* desc, const uint1
     a.part_ml = static_cast<float2*>(workspace);
     a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + at);
   }
-  if (p.few) {
-    const int rc2 = diff_decode_launch(a, p.splits, s);
-    return rc2 || p.splits == 1 ? rc2 : diff_combine_launch(a, p.splits, s);
-  }
-  const int64_t jobs = static_cast<int64_t>(d.batch) * d.heads * d.q_len;
-  if ((jobs + 3) / 4 > 0x7fffffff) return bad("too many queries");
-  const unsigned grid = static_cast<unsigned>((jobs + 3) / 4);
-  if (d.head_dim == 64) diff_simple_kernel<64><<<grid, 128, 0, s>>>(a);
-  else diff_simple_kernel<32><<<grid, 128, 0, s>>>(a);
-  return check_cuda(cudaGetLastError(), "differential attention launch");
+  const int rc2 = p.few ? diff_decode_launch(a, p.splits, s) : diff_tc_launch(a, p.splits, status, s);
+  return rc2 || p.splits == 1 ? rc2 : diff_combine_launch(a, p.splits, s);
 }
 
 extern "C" int kb_diff_lambda(const float* q1, const float* k1, const float* q2, const float* k2, int heads,

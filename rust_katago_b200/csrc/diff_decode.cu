@@ -73,7 +73,8 @@ __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 
 
 // NR: 8-row tiles per warp.
 template <int D, int NR, bool F16>
-__global__ void __launch_bounds__(32 * kWarps, NR == 1 ? 3 : 2) diff_decode_kernel(const DiffArgs a, int row_tiles) {
+__global__ void __launch_bounds__(32 * kWarps, NR == 1 ? 3 : 2) diff_decode_kernel(const DiffArgs a, int splits,
+                                                                                      int row_tiles) {
   constexpr int kCh = D / 32;   // 16-byte pieces per thread of a K row, and of half a V row
   constexpr int kKs = D / 16;   // steps of the score product
   constexpr int kMt = D / 8;    // 16-dim tiles of the value product
@@ -82,8 +83,8 @@ __global__ void __launch_bounds__(32 * kWarps, NR == 1 ? 3 : 2) diff_decode_kern
   const kb_diff_attention_desc& d = a.d;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int share = d.heads / d.kv_heads;
-  const int hk = blockIdx.y / row_tiles, r0 = (blockIdx.y % row_tiles) * kRows;
-  const int b = blockIdx.z, split = blockIdx.x, splits = gridDim.x;
+  const int split = blockIdx.x % splits, unit = blockIdx.x / splits;
+  const int hk = unit / row_tiles, r0 = (unit % row_tiles) * kRows, b = blockIdx.y;
   const int rows = min(kRows, d.q_len * share - r0);  // valid rows of this tile
 
   // Keys of the tile, of this split, and of each row held by this thread.
@@ -323,7 +324,7 @@ __global__ void __launch_bounds__(32 * kWarps, NR == 1 ? 3 : 2) diff_decode_kern
       }
     }
     if (splits == 1) {
-      finish_row<kE>(a, b, i, h, lane, acc, mm, ll);
+      finish_row<kE>(a, b, i, h, lane, acc, ll);
     } else {
       write_partial<kE>(a, splits, split, b, i, h, lane, acc, mm, ll);
     }
@@ -340,7 +341,12 @@ int launch(const DiffArgs& a, int splits, cudaStream_t s) {
     const int rc = smem_opt_in(reinterpret_cast<const void*>(kern), kBytes);
     if (rc) return rc;
   }
-  kern<<<dim3(splits, a.d.kv_heads * row_tiles, a.d.batch), 32 * kWarps, kBytes, s>>>(a, row_tiles);
+  const int64_t grid = static_cast<int64_t>(splits) * a.d.kv_heads * row_tiles;
+  if (grid > 0x7fffffff) {
+    set_error("kb_diff_attention: too many queries");
+    return KB_E_INVALID;
+  }
+  kern<<<dim3(static_cast<unsigned>(grid), a.d.batch), 32 * kWarps, kBytes, s>>>(a, splits, row_tiles);
   return check_cuda(cudaGetLastError(), "differential attention (few queries) launch");
 }
 

@@ -1,0 +1,629 @@
+// Differential attention of many queries on the tcgen05 tensor cores.
+//
+// Per pair of a query and a key it does 12 D flop and 2 exponentials: at D = 64
+// 0.094 clocks of an SM's tensor pipe against 0.125 of its special-function
+// unit (16 exponentials a clock), at D = 32 0.047 against 0.125, so the
+// softmax bounds it and the tensor cores have to be fed without holding it up.
+//
+// The two maps are what makes that easy: a block takes 128 queries of one head
+// and walks the keys in tiles of 128; each map has its own warpgroup of softmax
+// (one query per thread), its own accumulators and its own issuing warp, and
+// while one map's tile is in the tensor cores the other's is in the softmax.
+//   warps 0-3, 4-7   softmax of map 0, 1
+//   warps 8-11       epilogue: the weighted difference, its norm, the output
+//   warps 12, 13     MMA issue of map 0, 1
+//   warp 14          TMA loads of Q, K and V
+//   warp 15          key mask bits; clears the V rows of hidden keys
+//   shared memory    Q of two items, a ring of K tiles (both maps) and one of
+//                    V tiles (shared by the maps), swizzled as the MMAs read them
+//   tensor memory    S of each map (128 columns, overwritten by P as packed
+//                    16-bit pairs, the A operand of P V) and O of each map (2 D)
+// One pass over the keys with a running maximum and sum per map.  O is rescaled
+// only when a row's maximum grows by more than 2^8 (then by the softmax
+// warps, which at that point own it: S of a tile is issued after P V of the
+// tile before).  P is rounded to the 16-bit type; sums are taken of the
+// unrounded P in fp32.
+// V rows of keys that kv_lens or key_mask hide are cleared in shared memory:
+// their P is 0, but 0 * NaN is not.
+// When items are too few for the SMs, the keys of an item are split over blocks
+// and diff_combine joins the parts in a fixed order.
+#include <math.h>
+#include <stdint.h>
+
+#include <atomic>
+
+#include "kb_diff.cuh"
+#include "kb_internal.h"
+#include "kb_numeric.cuh"
+#include "kb_ptx.cuh"
+
+namespace kb {
+namespace {
+
+constexpr int kTile = 128;  // queries per item, keys per tile
+constexpr int kThreads = 512;
+constexpr uint32_t kTmemCols = 512;
+constexpr float kLazy = 8.0f;
+// Registers of the softmax, epilogue and issuing warpgroups: together the
+// 4 x 128 per thread that the block is launched with.
+constexpr int kRegsSoft = 176, kRegsEpi = 112, kRegsRest = 48;
+static_assert(2 * kRegsSoft + kRegsEpi + kRegsRest <= 4 * 128, "register split");
+
+template <int D>
+struct Geo {
+  static constexpr int kStages = D == 64 ? 2 : 4;
+  static constexpr int kQk = kTile * D * 2;         // one map's Q or K tile
+  static constexpr int kV = kTile * 2 * D * 2;      // V tile: 2 D / 64 columns of 128-byte rows
+  static constexpr int kVCol = kTile * 128;
+  static constexpr int kQOff = 0;                   // [2 items][2 maps]
+  static constexpr int kKOff = 4 * kQk;             // [stage][2 maps]
+  static constexpr int kVOff = kKOff + kStages * 2 * kQk;
+  static constexpr int kBarOff = kVOff + kStages * kV;
+  static constexpr int kBars = 512;
+  static constexpr int kMlOff = kBarOff + kBars;    // [2 maps][128] {m, l}
+  static constexpr int kMaskOff = kMlOff + 2 * kTile * 8;  // [stage][4] words
+  static constexpr int kBytes = kMaskOff + kStages * 16 + 1024;
+  static constexpr uint32_t kO = 256, kDv = 2 * D;  // TMEM: S at 0 and 128, O at kO and kO + kDv
+};
+
+struct Items {
+  int q_tiles, splits, count;
+};
+
+// 0 for a dimension that the strides broadcast (its tensor map extent is 1), else 1.
+struct Broadcast {
+  int q_batch, q_head, q_map, k_batch, k_head, k_map, v_batch, v_head;
+};
+
+// Item `at`: (b, h, q tile, split).  Causal: the last query tiles, which see
+// the most keys, first; otherwise the tiles of a head together, so that its K
+// and V come from L2.
+__device__ __forceinline__ void item_of(const DiffArgs& a, const Items& it, int at, int& b, int& h, int& qt, int& split) {
+  split = at % it.splits;
+  at /= it.splits;
+  if (a.d.causal) {
+    const int bh = a.d.batch * a.d.heads;
+    qt = it.q_tiles - 1 - at / bh;
+    at %= bh;
+  } else {
+    qt = at % it.q_tiles;
+    at /= it.q_tiles;
+  }
+  h = at % a.d.heads;
+  b = at / a.d.heads;
+}
+
+// Key tiles [t0, t1) of an item.
+__device__ __forceinline__ void tiles_of(const DiffArgs& a, const Items& it, int b, int qt, int split, int& n, int& t0,
+                                         int& t1) {
+  n = key_count(a, b);
+  int first, last;
+  key_range_n(a.d, n, qt * kTile, min(a.d.q_len, qt * kTile + kTile) - 1, first, last);
+  const int lo = first / kTile, hi = last > first ? (last + kTile - 1) / kTile : lo;
+  const int per = (hi - lo + it.splits - 1) / it.splits;
+  t0 = min(hi, lo + split * per);
+  t1 = min(hi, t0 + per);
+}
+
+template <int D>
+__device__ __forceinline__ uint64_t tile_desc(uint32_t saddr) {
+  if constexpr (D == 64) return sw128_desc(saddr);
+  else return sw64_desc(saddr);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
+
+// Bits [lo, hi) of a 32-bit word, lo and hi any integers.
+__device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
+  const uint32_t below_hi = hi >= 32 ? 0xffffffffu : hi <= 0 ? 0u : (1u << hi) - 1u;
+  const uint32_t below_lo = lo >= 32 ? 0xffffffffu : lo <= 0 ? 0u : (1u << lo) - 1u;
+  return below_hi & ~below_lo;
+}
+
+#define KB_WARP_WAIT(bar, parity) __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag))
+
+template <int D, bool F16>
+__global__ void __launch_bounds__(kThreads, 1) diff_tc_kernel(const __grid_constant__ CUtensorMap map_q,
+                                                              const __grid_constant__ CUtensorMap map_k,
+                                                              const __grid_constant__ CUtensorMap map_v,
+                                                              const __grid_constant__ DiffArgs a, const Items items,
+                                                              const Broadcast bc, unsigned* status) {
+  using G = Geo<D>;
+  constexpr int kS = G::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + G::kBarOff);
+  uint64_t* q_full = bars;            // [2] Q of an item landed              (tx bytes)
+  uint64_t* q_empty = bars + 2;       // [2] both maps' S MMAs read it        (2 commits)
+  uint64_t* s_full = bars + 4;        // [map] S ready                        (commit)
+  uint64_t* p_full = bars + 6;        // [map] P written                      (128 arrivals)
+  uint64_t* pv_done = bars + 8;       // [map] P V done: P consumed           (commit)
+  uint64_t* o_full = bars + 10;       // [map] O of an item complete          (commit)
+  uint64_t* o_empty = bars + 12;      // O, maxima and sums read              (128 arrivals)
+  uint64_t* ml_full = bars + 13;      // maxima and sums of an item written   (256 arrivals)
+  uint64_t* drain = bars + 14;        // [2] after an abort: issued MMAs done (commit)
+  uint64_t* k_full = bars + 16;       // [stage]                              (tx bytes)
+  uint64_t* k_empty = k_full + kS;    // [stage]                              (2 commits)
+  uint64_t* v_full = k_empty + kS;    // [stage]                              (tx bytes)
+  uint64_t* v_empty = v_full + kS;    // [stage]                              (2 commits)
+  uint64_t* v_ready = v_empty + kS;   // [stage] hidden rows cleared          (32 arrivals)
+  uint64_t* bits_full = v_ready + kS; // [stage] key mask bits written        (32 arrivals)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bits_full + kS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  static_assert((16 + 6 * kS) * 8 + 8 <= G::kBars, "barrier space");
+  float2* ml = reinterpret_cast<float2*>(smem + G::kMlOff);
+  uint32_t* mask_bits = reinterpret_cast<uint32_t*>(smem + G::kMaskOff);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 2);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], kTile);
+      mbar_init(&pv_done[i], 1);
+      mbar_init(&o_full[i], 1);
+      mbar_init(&drain[i], 1);
+    }
+    mbar_init(o_empty, kTile);
+    mbar_init(ml_full, 2 * kTile);
+    for (int i = 0; i < kS; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 2);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 2);
+      mbar_init(&v_ready[i], 32);
+      mbar_init(&bits_full[i], 32);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 12) {
+    tmem_alloc(tmem_slot, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const bool has_mask = a.key_mask != nullptr;
+
+  if (warp < 8) {
+    // ------------------------------------------------------------ softmax
+    regs_inc<kRegsSoft>();
+    const int map = warp >> 2;
+    const int row = threadIdx.x & (kTile - 1);
+    const uint32_t s_addr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + map * 128;
+    const uint32_t o_addr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + G::kO + map * G::kDv;
+    const float scale = a.scale_log2;
+    int tile = 0, busy = 0;  // tiles and items with tiles so far
+    bool ok = true;
+    for (int at = blockIdx.x; at < items.count && ok; at += gridDim.x) {
+      int b, h, qt, split, n, t0, t1;
+      item_of(a, items, at, b, h, qt, split);
+      tiles_of(a, items, b, qt, split, n, t0, t1);
+      if (t0 >= t1) continue;
+      int lo, hi, common_lo, common_hi, x0, x1;
+      const int i0 = qt * kTile, i1 = min(a.d.q_len, i0 + kTile) - 1, i = min(i0 + row, i1);
+      key_range_n(a.d, n, i, i, lo, hi);
+      key_range_n(a.d, n, i1, i1, common_lo, x1);
+      key_range_n(a.d, n, i0, i0, x0, common_hi);
+      float m = -INFINITY, l = 0.0f;
+      for (int t = t0; t < t1; ++t, ++tile) {
+        const int stage = tile % kS;
+        const bool inside = !has_mask && t * kTile >= common_lo && t * kTile + kTile <= common_hi;
+        if (!KB_WARP_WAIT(&s_full[map], tile & 1) ||
+            (has_mask && !KB_WARP_WAIT(&bits_full[stage], (tile / kS) & 1))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t s[128];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(s + 32 * c));
+        tmem_ld_wait();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld_wait(*reinterpret_cast<uint32_t(*)[32]>(s + 32 * c));
+        if (!inside) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int base = t * kTile + 32 * c;
+            uint32_t see = bits_between(lo - base, hi - base);
+            if (has_mask) see &= mask_bits[stage * 4 + c];
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (!(see >> k & 1u)) s[32 * c + k] = 0xff800000u;
+          }
+        }
+        float top[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          top[c] = fmaxf(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1]));
+#pragma unroll
+          for (int k = 1; k < 16; ++k)
+            top[c] = max3(top[c], __uint_as_float(s[8 * k + 2 * c]), __uint_as_float(s[8 * k + 2 * c + 1]));
+        }
+        const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
+        const bool grow = now > m + kLazy || (m == -INFINITY && now > -INFINITY);
+        if (__any_sync(0xffffffffu, grow)) {
+          const float next = fmaxf(m, now);
+          const float f = m == -INFINITY ? 1.0f : ex2(m - next);  // sums are 0 before the first key
+          m = next;
+          l *= f;
+          if (t > t0) {
+#pragma unroll
+            for (int c = 0; c < static_cast<int>(G::kDv) / 16; ++c) {
+              uint32_t o[16];
+              tmem_ld16(o_addr + 16 * c, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+              tmem_st16(o_addr + 16 * c, o);
+            }
+          }
+        }
+        const float base = m == -INFINITY ? 0.0f : m;
+        float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            const float2 x = fma2(make_float2(__uint_as_float(s[32 * c + 2 * k]), __uint_as_float(s[32 * c + 2 * k + 1])),
+                                  make_float2(scale, scale), make_float2(-base, -base));
+            const float2 p = make_float2(ex2(x.x), ex2(x.y));
+            sum[k & 1] = add2(sum[k & 1], p);
+            pk[k] = pack16x2(p, F16);
+          }
+          tmem_st16(s_addr + 16 * c, pk);
+        }
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&p_full[map]);
+      }
+      if (!ok) break;
+      // The epilogue has read the previous item's maxima and sums.
+      if (busy > 0 && !KB_WARP_WAIT(o_empty, (busy - 1) & 1)) break;
+      ml[map * kTile + row] = make_float2(m, l);
+      mbar_arrive(ml_full);
+      ++busy;
+    }
+  } else if (warp < 12) {
+    // ------------------------------------------------------------ epilogue
+    regs_dec<kRegsEpi>();
+    const int row = threadIdx.x & (kTile - 1);
+    const uint32_t o_addr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + G::kO;
+    int busy = 0;
+    for (int at = blockIdx.x; at < items.count; at += gridDim.x) {
+      int b, h, qt, split, n, t0, t1;
+      item_of(a, items, at, b, h, qt, split);
+      tiles_of(a, items, b, qt, split, n, t0, t1);
+      const int i = qt * kTile + row;
+      const bool live = i < a.d.q_len;
+      const bool any = t0 < t1;
+      float2 v0 = make_float2(-INFINITY, 0.0f), v1 = v0;
+      if (any) {
+        if (!KB_WARP_WAIT(ml_full, busy & 1) || !KB_WARP_WAIT(&o_full[0], busy & 1) ||
+            !KB_WARP_WAIT(&o_full[1], busy & 1))
+          break;
+        tc_fence_after();
+        v0 = ml[row], v1 = ml[kTile + row];
+      }
+      if (items.splits > 1) {
+        const int64_t at2 = live ? (row_index(a, b, i, h) * items.splits + split) * 2 : 0;
+        if (live) a.part_ml[at2] = v0, a.part_ml[at2 + 1] = v1;
+        if (any) {
+#pragma unroll 1
+          for (int c = 0; c < 2 * static_cast<int>(G::kDv) / 32; ++c) {  // O of map 0, then of map 1
+            uint32_t o[32];
+            tmem_ld32(o_addr + 32 * c, o);
+            tmem_ld_wait(o);
+            if (live) {
+              float4* dst = reinterpret_cast<float4*>(a.part_o + at2 * G::kDv + 32 * c);
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                dst[k] = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]),
+                                     __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
+            }
+          }
+        }
+      } else {
+        const float w0 = v0.y == 0.0f ? 0.0f : 1.0f / v0.y;
+        const float w1 = v1.y == 0.0f ? 0.0f : a.lambda[h] / v1.y;
+        uint16_t* out = a.out + b * a.d.out_batch + i * a.d.out_token + h * a.d.out_head;
+        float f = a.d.out_scale;
+        if (any && a.gamma) {
+          float ss = 0.0f;
+#pragma unroll 1
+          for (int c = 0; c < static_cast<int>(G::kDv) / 32; ++c) {
+            uint32_t o0[32], o1[32];
+            tmem_ld32(o_addr + 32 * c, o0);
+            tmem_ld32(o_addr + G::kDv + 32 * c, o1);
+            tmem_ld_wait(o0);
+            tmem_ld_wait(o1);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              const float r = __uint_as_float(o0[k]) * w0 - __uint_as_float(o1[k]) * w1;
+              ss = fmaf(r, r, ss);
+            }
+          }
+          f *= 1.0f / sqrtf(ss / static_cast<float>(G::kDv) + a.d.eps);
+        }
+#pragma unroll 1
+        for (int c = 0; c < static_cast<int>(G::kDv) / 32; ++c) {
+          uint32_t o0[32], o1[32], w[16];
+          if (any) {
+            tmem_ld32(o_addr + 32 * c, o0);
+            tmem_ld32(o_addr + G::kDv + 32 * c, o1);
+            tmem_ld_wait(o0);
+            tmem_ld_wait(o1);
+          }
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            float2 r = make_float2(0.0f, 0.0f);
+            if (any) {
+              r.x = (__uint_as_float(o0[2 * k]) * w0 - __uint_as_float(o1[2 * k]) * w1) * f;
+              r.y = (__uint_as_float(o0[2 * k + 1]) * w0 - __uint_as_float(o1[2 * k + 1]) * w1) * f;
+              if (a.gamma) r.x *= a.gamma[32 * c + 2 * k], r.y *= a.gamma[32 * c + 2 * k + 1];
+            }
+            w[k] = pack16x2(r, F16);
+          }
+          if (live) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              *reinterpret_cast<uint4*>(out + 32 * c + 8 * k) = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+          }
+        }
+      }
+      if (any) {
+        tc_fence_before();
+        mbar_arrive(o_empty);
+        ++busy;
+      }
+    }
+  } else {
+    regs_dec<kRegsRest>();
+    if (warp < 14) {
+      // ---------------------------------------------------------- MMA issue of one map
+      if (lane == 0) {
+        const int map = warp - 12;
+        constexpr uint32_t kFmt = F16 ? 0u : 1u;
+        constexpr uint32_t kId = (1u << 4) | (kFmt << 7) | (kFmt << 10) | (static_cast<uint32_t>(128 >> 4) << 24);
+        constexpr uint32_t kIdS = kId | (static_cast<uint32_t>(kTile >> 3) << 17);
+        constexpr uint32_t kIdV = kId | (1u << 16) /* B MN-major */ | (G::kDv >> 3 << 17);
+        const uint32_t s_tmem = tmem + map * 128, o_tmem = tmem + G::kO + map * G::kDv;
+        int tile = 0, busy = 0;
+        bool ok = true;
+        for (int at = blockIdx.x; at < items.count && ok; at += gridDim.x) {
+          int b, h, qt, split, n, t0, t1;
+          item_of(a, items, at, b, h, qt, split);
+          tiles_of(a, items, b, qt, split, n, t0, t1);
+          if (t0 >= t1) continue;
+          const uint64_t qdesc = tile_desc<D>(smem_u32(smem + G::kQOff + ((busy & 1) * 2 + map) * G::kQk));
+          ok = mbar_wait(&q_full[busy & 1], (busy >> 1) & 1, abort_flag);
+          for (int t = t0; t < t1 && ok; ++t, ++tile) {
+            const int stage = tile % kS;
+            // S overwrites the P of the tile before
+            ok = (tile == 0 || mbar_wait(&pv_done[map], (tile - 1) & 1, abort_flag)) &&
+                 mbar_wait(&k_full[stage], (tile / kS) & 1, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t kdesc = tile_desc<D>(smem_u32(smem + G::kKOff + (stage * 2 + map) * G::kQk));
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+              mma_issue<kKindBF16>(s_tmem, qdesc + 2 * k, kdesc + 2 * k, kIdS, k != 0, 0, 0);
+            tc_commit(&s_full[map]);
+            tc_commit(&k_empty[stage]);
+            if (t == t1 - 1) tc_commit(&q_empty[busy & 1]);
+            ok = mbar_wait(&v_ready[stage], (tile / kS) & 1, abort_flag) &&
+                 mbar_wait(&p_full[map], tile & 1, abort_flag) &&
+                 (t > t0 || busy == 0 || mbar_wait(o_empty, (busy - 1) & 1, abort_flag));
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t vdesc = sw128_mn_desc(smem_u32(smem + G::kVOff + stage * G::kV), G::kVCol);
+#pragma unroll
+            for (int k = 0; k < kTile / 16; ++k)
+              mma_f16_ts(o_tmem, s_tmem + 8 * k, vdesc + static_cast<uint64_t>(k * 16 * 128 >> 4), kIdV,
+                         t > t0 || k != 0);
+            tc_commit(&pv_done[map]);
+            tc_commit(&v_empty[stage]);
+            if (t == t1 - 1) tc_commit(&o_full[map]);
+          }
+          ++busy;
+        }
+        if (*abort_flag) {  // let the MMAs issued so far finish before tensor memory goes
+          int none = 0;
+          tc_commit(&drain[map]);
+          mbar_wait(&drain[map], 0, &none);
+        }
+      }
+    } else if (warp == 14) {
+      // ---------------------------------------------------------- TMA loads
+      if (lane == 0) {
+        tma_prefetch_desc(&map_q);
+        tma_prefetch_desc(&map_k);
+        tma_prefetch_desc(&map_v);
+        const int share = a.d.heads / a.d.kv_heads;
+        int tile = 0, tile_v = 0, busy = 0;  // K tiles, V tiles and items loaded
+        bool ok = true;
+        for (int at = blockIdx.x; at < items.count && ok; at += gridDim.x) {
+          int b, h, qt, split, n, t0, t1;
+          item_of(a, items, at, b, h, qt, split);
+          tiles_of(a, items, b, qt, split, n, t0, t1);
+          if (t0 >= t1) continue;
+          const int hk = h / share, qb = busy & 1;
+          ok = mbar_wait(&q_empty[qb], ((busy >> 1) & 1) ^ 1, abort_flag);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&q_full[qb], 2 * G::kQk);
+          for (int m = 0; m < 2; ++m)
+            tma_load_5d(smem + G::kQOff + (qb * 2 + m) * G::kQk, &map_q, &q_full[qb], 0, qt * kTile, h * bc.q_head,
+                        m * bc.q_map, b * bc.q_batch);
+          ++busy;
+          for (int t = t0; t < t1; ++t) {
+            const int stage = tile % kS;
+            const uint32_t parity = ((tile / kS) & 1) ^ 1;
+            ok = mbar_wait(&k_empty[stage], parity, abort_flag);
+            if (!ok) break;
+            mbar_arrive_expect_tx(&k_full[stage], 2 * G::kQk);
+            for (int m = 0; m < 2; ++m)
+              tma_load_5d(smem + G::kKOff + (stage * 2 + m) * G::kQk, &map_k, &k_full[stage], 0, t * kTile,
+                          hk * bc.k_head, m * bc.k_map, b * bc.k_batch);
+            ++tile;
+            ok = mbar_wait(&v_empty[stage], parity, abort_flag);
+            if (!ok) break;
+            mbar_arrive_expect_tx(&v_full[stage], G::kV);
+            for (int c = 0; c < static_cast<int>(G::kDv) / 64; ++c)
+              tma_load_4d(smem + G::kVOff + stage * G::kV + c * G::kVCol, &map_v, &v_full[stage], 64 * c, t * kTile,
+                          hk * bc.v_head, b * bc.v_batch);
+            ++tile_v;
+          }
+        }
+        if (*abort_flag) {  // let the copies issued so far land before shared memory goes
+          int none = 0;
+          for (int u = busy > 2 ? busy - 2 : 0; u < busy; ++u) mbar_wait(&q_full[u & 1], (u >> 1) & 1, &none);
+          for (int u = tile > kS ? tile - kS : 0; u < tile; ++u) mbar_wait(&k_full[u % kS], (u / kS) & 1, &none);
+          for (int u = tile_v > kS ? tile_v - kS : 0; u < tile_v; ++u) mbar_wait(&v_full[u % kS], (u / kS) & 1, &none);
+        }
+      }
+    } else {
+      // ---------------------------------------------------------- hidden keys
+      int tile = 0;
+      bool ok = true;
+      for (int at = blockIdx.x; at < items.count && ok; at += gridDim.x) {
+        int b, h, qt, split, n, t0, t1;
+        item_of(a, items, at, b, h, qt, split);
+        tiles_of(a, items, b, qt, split, n, t0, t1);
+        const uint8_t* mask = has_mask ? a.key_mask + b * a.d.mask_batch : nullptr;
+        for (int t = t0; t < t1; ++t, ++tile) {
+          const int stage = tile % kS;
+          const uint32_t parity = (tile / kS) & 1;
+          uint32_t see[4];
+          if (!KB_WARP_WAIT(&v_empty[stage], parity ^ 1)) {
+            ok = false;
+            break;
+          }
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int key = t * kTile + 32 * c + lane;
+            see[c] = __ballot_sync(0xffffffffu, key < n && (!has_mask || mask[key] != 0));
+          }
+          if (has_mask) {
+            if (lane < 4) mask_bits[stage * 4 + lane] = lane == 0 ? see[0] : lane == 1 ? see[1] : lane == 2 ? see[2] : see[3];
+            mbar_arrive(&bits_full[stage]);
+          }
+          if (!KB_WARP_WAIT(&v_full[stage], parity)) {
+            ok = false;
+            break;
+          }
+          uint8_t* v = smem + G::kVOff + stage * G::kV;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            if (see[c] == 0xffffffffu) continue;
+            // four rows at a time, 8 lanes a row; swizzling stays within a row
+            for (int r = lane >> 3; r < 32; r += 4)
+              if (!(see[c] >> r & 1u))
+                for (int col = 0; col < static_cast<int>(G::kDv) / 64; ++col)
+                  *reinterpret_cast<uint4*>(v + col * G::kVCol + (32 * c + r) * 128 + (lane & 7) * 16) =
+                      make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          mbar_arrive(&v_ready[stage]);
+        }
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (threadIdx.x == 0 && *abort_flag) record_status(status, KB_STATUS_TIMEOUT, KB_NO_LAYER);
+  if (warp == 12) tmem_dealloc(tmem, kTmemCols);
+}
+
+#undef KB_WARP_WAIT
+
+// Tensor map of 16-bit rows [.., token, `width`]: boxes of `box` columns by
+// kTile tokens.  `strides` and `extents` of the dimensions after the token;
+// broadcast ones collapse to extent 1 (flag 0).
+int encode(CUtensorMap* map, const void* base, int width, int box, long tokens, int64_t token_stride, int more,
+           const int64_t* strides, const long* extents, int* const* flags) {
+  long dims[5] = {width, tokens, 1, 1, 1}, bytes[4];
+  const int boxes[5] = {box, kTile, 1, 1, 1};
+  bytes[0] = tokens > 1 ? token_stride * 2 : width * 2;
+  for (int i = 0; i < more; ++i) {
+    const bool steps = extents[i] > 1 && strides[i] != 0;
+    *flags[i] = steps;
+    dims[2 + i] = steps ? extents[i] : 1;
+    bytes[1 + i] = steps ? strides[i] * 2 : width * 2;
+  }
+  const CUtensorMapSwizzle swz = box == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+  return encode_nd(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, base, 2 + more, dims, bytes, boxes, swz);
+}
+
+template <int D, bool F16>
+int launch(const DiffArgs& a, int splits, unsigned* status, cudaStream_t s) {
+  auto kern = diff_tc_kernel<D, F16>;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  static std::atomic<uint64_t> configured{0};
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(configured.load() & bit)) {
+    // The warpgroups trade registers: the launch has to hold all of them.
+    cudaFuncAttributes attr;
+    int rc = check_cuda(cudaFuncGetAttributes(&attr, kern), "differential attention attributes");
+    if (rc) return rc;
+    if (attr.numRegs * kThreads < 128 * (2 * kRegsSoft + kRegsEpi + kRegsRest)) {
+      set_error("differential attention: the kernel was built with too few registers for its split");
+      return KB_E_UNSUPPORTED;
+    }
+    rc = smem_opt_in(reinterpret_cast<const void*>(kern), Geo<D>::kBytes);
+    if (rc) return rc;
+    configured.fetch_or(bit);
+  }
+  const kb_diff_attention_desc& d = a.d;
+  Broadcast bc;
+  CUtensorMap mq, mk, mv;
+  const int64_t qs[3] = {d.q_head, d.q_map, d.q_batch}, ks[3] = {d.k_head, d.k_map, d.k_batch},
+                vs[2] = {d.v_head, d.v_batch};
+  const long qe[3] = {d.heads, 2, d.batch}, ke[3] = {d.kv_heads, 2, d.batch}, ve[2] = {d.kv_heads, d.batch};
+  int* const qf[3] = {&bc.q_head, &bc.q_map, &bc.q_batch};
+  int* const kf[3] = {&bc.k_head, &bc.k_map, &bc.k_batch};
+  int* const vf[2] = {&bc.v_head, &bc.v_batch};
+  int rc = encode(&mq, a.q, D, D, d.q_len, d.q_token, 3, qs, qe, qf);
+  if (!rc) rc = encode(&mk, a.k, D, D, d.kv_len, d.k_token, 3, ks, ke, kf);
+  if (!rc) rc = encode(&mv, a.v, 2 * D, 64, d.kv_len, d.v_token, 2, vs, ve, vf);
+  if (rc) return rc;
+  Items it;
+  it.q_tiles = (d.q_len + kTile - 1) / kTile;
+  it.splits = splits;
+  const int64_t count = static_cast<int64_t>(d.batch) * d.heads * it.q_tiles * splits;
+  if (count > 0x7fffffff - 1024) {
+    set_error("kb_diff_attention: too many query tiles");
+    return KB_E_INVALID;
+  }
+  it.count = static_cast<int>(count);
+  const int grid = it.count < num_sms(dev) ? it.count : num_sms(dev);
+  kern<<<grid, kThreads, Geo<D>::kBytes, s>>>(mq, mk, mv, a, it, bc, status);
+  return check_cuda(cudaGetLastError(), "differential attention launch");
+}
+
+}  // namespace
+
+int diff_tc_launch(const DiffArgs& a, int splits, unsigned* status, cudaStream_t s) {
+  const bool f16 = a.d.dtype == KB_DT_F16;
+  if (a.d.head_dim == 64) return f16 ? launch<64, true>(a, splits, status, s) : launch<64, false>(a, splits, status, s);
+  return f16 ? launch<32, true>(a, splits, status, s) : launch<32, false>(a, splits, status, s);
+}
+
+}  // namespace kb

@@ -1160,6 +1160,31 @@ int encode_3d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, long d
   return KB_OK;
 }
 
+int encode_nd(CUtensorMap* map, CUtensorMapDataType dt, const void* base, int rank, const long* dims,
+              const long* stride_bytes, const int* boxes, CUtensorMapSwizzle swz) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) {
+    set_error("cuTensorMapEncodeTiled is unavailable from the CUDA driver");
+    return KB_E_CUDA;
+  }
+  cuuint64_t d[5], strides[4];
+  cuuint32_t box[5], estr[5];
+  for (int i = 0; i < rank; ++i) {
+    d[i] = static_cast<cuuint64_t>(dims[i]);
+    box[i] = static_cast<cuuint32_t>(boxes[i]);
+    estr[i] = 1;
+    if (i > 0) strides[i - 1] = static_cast<cuuint64_t>(stride_bytes[i - 1]);
+  }
+  CUresult r = fn(map, dt, static_cast<cuuint32_t>(rank), const_cast<void*>(base), d, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled (" + std::to_string(rank) + "-D) failed (code " + std::to_string(int(r)) + ")");
+    return KB_E_CUDA;
+  }
+  return KB_OK;
+}
+
 int gemm_pick_bn(int kind, int epi, int m, int n) {
   (void)kind;
   if (epi == kEpiSwiGLU16) return 256;

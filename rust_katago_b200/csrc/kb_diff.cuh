@@ -64,13 +64,13 @@ __device__ __forceinline__ int64_t row_index(const DiffArgs& a, int b, int i, in
   return (static_cast<int64_t>(b) * a.d.q_len + i) * a.d.heads + h;
 }
 
-// A row's result from both maps' sums `acc` (kE dims per lane, dims lane kE..),
-// maxima and weights: the weighted difference, its norm, one rounding.  Whole warps.
+// A row's result from both maps' sums `acc` (kE dims per lane, dims lane kE..)
+// and weights `ll`: the weighted difference, its norm, one rounding.  Whole warps.
 template <int kE>
 __device__ __forceinline__ void finish_row(const DiffArgs& a, int b, int i, int h, int lane, const float (&acc)[2][kE],
-                                           const float (&mm)[2], const float (&ll)[2]) {
-  const float w0 = mm[0] == -INFINITY ? 0.0f : 1.0f / ll[0];
-  const float w1 = mm[1] == -INFINITY ? 0.0f : a.lambda[h] / ll[1];
+                                           const float (&ll)[2]) {
+  const float w0 = ll[0] == 0.0f ? 0.0f : 1.0f / ll[0];  // 0: no key was seen
+  const float w1 = ll[1] == 0.0f ? 0.0f : a.lambda[h] / ll[1];
   float r[kE], ss = 0.0f;
 #pragma unroll
   for (int e = 0; e < kE; ++e) {
@@ -108,6 +108,7 @@ __device__ __forceinline__ void write_partial(const DiffArgs& a, int splits, int
 }
 
 int diff_decode_launch(const DiffArgs& a, int splits, cudaStream_t s);
+int diff_tc_launch(const DiffArgs& a, int splits, unsigned* status, cudaStream_t s);
 int diff_combine_launch(const DiffArgs& a, int splits, cudaStream_t s);
 int smem_opt_in(const void* kernel, int bytes);
 

@@ -118,6 +118,10 @@ int encode_2d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, long c
 int encode_3d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, long d0, long d1, long d2, long stride1_bytes,
               long stride2_bytes, int box0, int box1, int box2, CUtensorMapSwizzle swz);
 
+// Tensor map of rank 2..5: dims (innermost first), byte strides of dims 1.., box extents.
+int encode_nd(CUtensorMap* map, CUtensorMapDataType dt, const void* base, int rank, const long* dims,
+              const long* stride_bytes, const int* boxes, CUtensorMapSwizzle swz);
+
 // Columns per N tile chosen for a given N (the SwiGLU dual-weight packing
 // depends on it).
 int gemm_pick_bn(int kind, int epi, int m, int n);

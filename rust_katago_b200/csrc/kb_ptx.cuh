@@ -122,6 +122,24 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, u
       : "memory");
 }
 
+// 4-D and 5-D tiled loads; x is a multiple of 16 bytes at every call site.
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z,
+                                            int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z,
+                                            int w, int v) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v)
+      : "memory");
+}
+
 // Prefetch a 2-D tile of a tensor map into L2 (no shared memory, no completion).
 __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(
@@ -241,6 +259,19 @@ __device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr) {
   d |= static_cast<uint64_t>(1024 >> 4) << 32;            // stride offset between 8-row groups
   d |= static_cast<uint64_t>(1) << 46;                    // descriptor version for sm_100
   d |= static_cast<uint64_t>(2) << 61;                    // SWIZZLE_128B
+  return d;
+}
+
+// A [K rows, N x 16-bit] operand in MN-major order, N a multiple of 64: 64-wide
+// columns of 128-byte rows with the 128-byte swizzle (a TMA box each),
+// `column_bytes` apart; rows in 8-row core groups of 1024 bytes.
+__device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t saddr, uint32_t column_bytes) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4);      // start address
+  d |= static_cast<uint64_t>(column_bytes >> 4) << 16;        // leading offset: between 64-wide columns
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;                // stride offset between 8-row groups
+  d |= static_cast<uint64_t>(1) << 46;                        // descriptor version for sm_100
+  d |= static_cast<uint64_t>(2) << 61;                        // SWIZZLE_128B
   return d;
 }
 
@@ -380,6 +411,13 @@ __device__ __forceinline__ void tmem_st1(uint32_t taddr, uint32_t r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(r) : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Move registers between the warpgroups of a block; every warp of a warpgroup
+// executes the same one.  The groups' shares must not exceed the launch's total.
+template <int N>
+__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 // Record an error in a sticky status word [flags, first_layer]: flags are OR-ed,
 // the first reporting layer wins.
