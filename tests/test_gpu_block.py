@@ -304,6 +304,9 @@ CASES = [
     (1, 33, 9000, 4, 4, 32, True, 0, [8999], "random"),
     (1, 1, 20000, 2, 2, 64, True, 0, None, "random"),
     (2, 1, 5000, 16, 1, 64, True, 700, [5000, 512], "random"),
+    # several tiles of queries for every SM
+    (40, 361, 361, 6, 6, 32, False, 0, None, "random"),
+    (24, 300, 333, 8, 2, 64, True, 150, None, None),
 ]
 
 
@@ -433,9 +436,9 @@ def test_empty_lengths(cuda):
     assert torch.equal(got[0], block.diff_attention(q, k, v, lam)[0]) and (got[1] == 0).all()
 
 
-@pytest.mark.parametrize("q_len,kv_len", [(1, 30000), (361, 361), (100, 6000)])
-def test_repeats_are_bitwise_equal_on_any_stream(cuda, q_len, kv_len):
-    q, k, v, lam, gamma = attn_inputs(1, q_len, kv_len, 2, 2, 64, torch.bfloat16)
+@pytest.mark.parametrize("batch,q_len,kv_len", [(1, 1, 30000), (1, 361, 361), (1, 100, 6000), (130, 361, 361), (1, 9000, 9000)])
+def test_repeats_are_bitwise_equal_on_any_stream(cuda, batch, q_len, kv_len):
+    q, k, v, lam, gamma = attn_inputs(batch, q_len, kv_len, 2, 2, 64, torch.bfloat16)
     ref = block.diff_attention(q, k, v, lam, gamma=gamma, causal=True)
     status = torch.tensor([0, -1], dtype=torch.int32, device="cuda")
     side = torch.cuda.Stream()
