@@ -5,29 +5,24 @@
 // unit (16 exponentials a clock), at D = 32 0.047 against 0.125, so the
 // softmax bounds it and the tensor cores have to be fed without holding it up.
 //
-// A block takes 128 queries of one head and walks the keys in tiles of 128, by
-// halves of 64.  Each map has its own accumulators, its own issuing warps, S of
-// two halves and two warpgroups of softmax (one query per thread) that take the
-// halves in turn: while some warps wait for their scores (P V of a half and S
-// of the half after next are a chain of about 1,000 clocks), take maxima or
-// store P, others keep the special-function unit busy.  With one warpgroup per
-// map the same chain was exposed every time: 4,200 clocks per 128 keys with
-// one S of 128 keys, 3,900 with two S of 64, 4,400 with explicit turns.
-//   warps 0-7, 8-15  softmax of map 0, 1: four warps for each parity of halves
-//   warps 16-19      epilogue: the weighted difference, its norm, the output
-//   warps 20, 21     issue of S of map 0, 1
-//   warps 22, 23     issue of P V of map 0, 1 (with one warp for both products
-//                    of a map its waits alone took 2,200 clocks per half)
-//   warp 24          TMA loads of Q, K and V
-//   warp 25          key mask bits; clears the V rows of hidden keys
+// A block takes 128 queries of one head and walks the keys in tiles of 128.
+// Each map has its own warpgroup of softmax (one query per thread) and its own
+// S and O; one warp issues the products of both in strict turns, P V and the
+// next S of map 0, then those of map 1, which keeps the maps half a step apart:
+// while one is in the tensor cores the other is in its exponentials.
+//   warps 0-3, 4-7   softmax of map 0, 1
+//   warps 8-11       epilogue: the weighted difference, its norm, the output
+//   warp 12          MMA issue
+//   warp 13          TMA loads of Q, K and V
+//   warp 14          key mask bits; clears the V rows of hidden keys
 //   shared memory    Q of two items, a ring of K tiles (both maps) and one of
 //                    V tiles (shared by the maps), swizzled as the MMAs read them
-//   tensor memory    two S of each map (64 columns each, overwritten by P as
-//                    packed 16-bit pairs, the A operand of P V), O of each map (2 D)
-// One pass over the keys with a running maximum per map, handed from half to
-// half through shared memory, and a running sum per warpgroup.  O is rescaled
+//   tensor memory    S of each map (128 columns, overwritten by P as packed
+//                    16-bit pairs, the A operand of P V) and O of each map (2 D)
+// One pass over the keys with a running maximum and sum per map.  O is rescaled
 // only when a row's maximum grows by more than 2^8 (then by the softmax
-// warps, once P V of the half before is done).  P is rounded to the 16-bit type; sums are taken of the
+// warps, which at that point own it: S of a tile is issued after P V of the
+// tile before is done).  P is rounded to the 16-bit type; sums are taken of the
 // unrounded P in fp32.
 // V rows of keys that kv_lens or key_mask hide are cleared in shared memory:
 // their P is 0, but 0 * NaN is not.
@@ -47,15 +42,16 @@ namespace kb {
 namespace {
 
 constexpr int kTile = 128;  // queries per item, keys per tile
-constexpr int kHalf = 64;   // keys per S
-constexpr int kThreads = 896;
-constexpr int kEpiWarp = 16, kScoreWarp = 20, kValueWarp = 22, kLoadWarp = 24, kHiddenWarp = 25;
+constexpr int kFirst = 96;  // keys of the first of the two parts of P
+constexpr int kThreads = 512;
+constexpr int kEpiWarp = 8, kMmaWarp = 12, kLoadWarp = 13, kHiddenWarp = 14;
 constexpr uint32_t kTmemCols = 512;
 constexpr float kLazy = 8.0f;
 // Registers of the softmax, epilogue and issuing warpgroups: together the
-// 7 x 72 per thread that the block is launched with.
-constexpr int kRegsLaunch = 72, kRegsSoft = 80, kRegsEpi = 72, kRegsRest = 56;
-static_assert(4 * kRegsSoft + kRegsEpi + 2 * kRegsRest <= 7 * kRegsLaunch, "register split");
+// 4 x 128 per thread that the block is launched with.
+constexpr int kRegsLaunch = 128, kRegsSoft = 184, kRegsEpi = 88, kRegsRest = 56;
+static_assert(2 * kRegsSoft + kRegsEpi + kRegsRest <= 4 * kRegsLaunch && kRegsLaunch * kThreads <= 65536,
+              "register split");
 
 template <int D>
 struct Geo {
@@ -67,10 +63,9 @@ struct Geo {
   static constexpr int kKOff = 4 * kQk;             // [stage][2 maps]
   static constexpr int kVOff = kKOff + kStages * 2 * kQk;
   static constexpr int kBarOff = kVOff + kStages * kV;
-  static constexpr int kBars = 768;
-  static constexpr int kMlOff = kBarOff + kBars;    // [2 maps][2 parities][128] {m, l}
-  static constexpr int kMOff = kMlOff + 4 * kTile * 8;     // [2 maps][2 parities][128] m after a half
-  static constexpr int kMaskOff = kMOff + 4 * kTile * 4;   // [stage][4] words
+  static constexpr int kBars = 512;
+  static constexpr int kMlOff = kBarOff + kBars;    // [2 maps][128] {m, l}
+  static constexpr int kMaskOff = kMlOff + 2 * kTile * 8;  // [stage][4] words
   static constexpr int kBytes = kMaskOff + kStages * 16 + 1024;
   static constexpr uint32_t kO = 256, kDv = 2 * D;  // TMEM: S of map m at 128 m, O at kO + m kDv
 };
@@ -102,17 +97,16 @@ __device__ __forceinline__ void item_of(const DiffArgs& a, const Items& it, int 
   b = at / a.d.heads;
 }
 
-// Halves [u0, u1) of the keys of an item (u0 is even: whole tiles from there).
-__device__ __forceinline__ void halves_of(const DiffArgs& a, const Items& it, int b, int qt, int split, int& n, int& u0,
-                                          int& u1) {
+// Key tiles [t0, t1) of an item.
+__device__ __forceinline__ void tiles_of(const DiffArgs& a, const Items& it, int b, int qt, int split, int& n, int& t0,
+                                         int& t1) {
   n = key_count(a, b);
   int first, last;
   key_range_n(a.d, n, qt * kTile, min(a.d.q_len, qt * kTile + kTile) - 1, first, last);
-  const int lo = first / kTile * 2, hi = last > first ? (last + kHalf - 1) / kHalf : lo;
-  const int per = ((hi - lo + it.splits - 1) / it.splits + 1) / 2 * 2;
-  u0 = min(hi, lo + split * per);
-  u1 = min(hi, u0 + per);
-  if (u0 >= u1) u0 = u1 = 0;
+  const int lo = first / kTile, hi = last > first ? (last + kTile - 1) / kTile : lo;
+  const int per = (hi - lo + it.splits - 1) / it.splits;
+  t0 = min(hi, lo + split * per);
+  t1 = min(hi, t0 + per);
 }
 
 // A block's items: one of each round of gridDim.x, from alternating ends, so
@@ -122,18 +116,18 @@ __device__ __forceinline__ int item_at(int round) {
          static_cast<int>(round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
 }
 
-// A walk over the halves of a block's items, for the roles that run ahead.
+// A walk over the tiles of a block's items, for the issuing warps.
 struct Walk {
-  int round, u, u0, u1;  // round of items, half, its item's halves
-  int item, tile;     // items and tiles before this one
+  int round, t, t0, t1;  // round of items, tile, its item's tiles
+  int item, tile;        // items and tiles before this one
   bool valid;
   __device__ __forceinline__ void seek(const DiffArgs& a, const Items& it) {
     for (int at; (at = item_at(round)) < it.count; ++round) {
       int split, n, b, h, qt;
       item_of(a, it, at, b, h, qt, split);
-      halves_of(a, it, b, qt, split, n, u0, u1);
-      if (u0 < u1) {
-        u = u0;
+      tiles_of(a, it, b, qt, split, n, t0, t1);
+      if (t0 < t1) {
+        t = t0;
         valid = true;
         return;
       }
@@ -144,12 +138,11 @@ struct Walk {
     round = 0, item = 0, tile = 0;
     seek(a, it);
   }
-  // This half is its tile's (its item's) last.
-  __device__ __forceinline__ bool ends_tile() const { return (u & 1) || u == u1 - 1; }
-  __device__ __forceinline__ bool ends_item() const { return u == u1 - 1; }
+  __device__ __forceinline__ bool begins_item() const { return t == t0; }
+  __device__ __forceinline__ bool ends_item() const { return t == t1 - 1; }
   __device__ __forceinline__ void step(const DiffArgs& a, const Items& it) {
-    tile += ends_tile();
-    if (++u < u1) return;
+    ++tile;
+    if (++t < t1) return;
     ++item;
     ++round;
     seek(a, it);
@@ -174,13 +167,6 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
   return r;
 }
 
-// One {maximum, sum} from those of the two parities of halves.
-__device__ __forceinline__ float2 joined(const float2& x, const float2& y) {
-  const float m = fmaxf(x.x, y.x);
-  const float fx = x.x == m ? 1.0f : ex2(x.x - m), fy = y.x == m ? 1.0f : ex2(y.x - m);
-  return make_float2(m, x.y * fx + y.y * fy);
-}
-
 // Bits [lo, hi) of a 32-bit word, lo and hi any integers.
 __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
   const uint32_t below_hi = hi >= 32 ? 0xffffffffu : hi <= 0 ? 0u : (1u << hi) - 1u;
@@ -188,16 +174,36 @@ __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
   return below_hi & ~below_lo;
 }
 
-// After an abort: let the MMAs that this thread has issued finish before
-// tensor memory is freed.
-__device__ __forceinline__ void drain_mmas(uint64_t* bar, volatile int* abort_flag) {
-  if (!*abort_flag) return;
-  int none = 0;
-  tc_commit(bar);
-  mbar_wait(bar, 0, &none);
+// mbar_wait in few instructions (it is inlined some thirty times, and the
+// kernel's loops have to stay in the instruction cache), without a hint of how
+// long to suspend: the default wakes sooner.  The limit is two seconds of the
+// timer's low word.
+__device__ __forceinline__ bool try_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool wait_short(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  if (try_wait(bar, parity)) return true;
+  uint32_t t0, t1;
+  asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t0));
+#pragma unroll 1
+  while (!try_wait(bar, parity)) {
+    asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t1));
+    if (t1 - t0 > static_cast<uint32_t>(kWaitLimitNs)) *abort_flag = 1;
+    if (*abort_flag) return false;
+  }
+  return true;
 }
 
-#define KB_WARP_WAIT(bar, parity) __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag))
+// The same for a whole warp, all lanes of which return what one would.
+#define KB_WARP_WAIT(bar, parity) __all_sync(0xffffffffu, wait_short(bar, parity, abort_flag))
 
 template <int D, bool F16>
 __global__ void __launch_bounds__(kThreads, 1) diff_tc_kernel(const __grid_constant__ CUtensorMap map_q,
@@ -211,219 +217,185 @@ __global__ void __launch_bounds__(kThreads, 1) diff_tc_kernel(const __grid_const
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + G::kBarOff);
   uint64_t* q_full = bars;            // [2] Q of an item landed              (tx bytes)
-  uint64_t* q_empty = bars + 2;       // [2] both maps' S MMAs read it        (2 commits)
-  uint64_t* s_full = bars + 4;        // [map][2] S ready                     (commit)
-  uint64_t* p_full = bars + 8;        // [map][2][part] 32 keys of P written  (128 arrivals)
-  // [map][2] P V done: P consumed (commit).  One per S buffer: with one per map
-  // P V of the next half could complete before a wait for this one began.
-  uint64_t* pv_done = bars + 16;
-  uint64_t* o_full = bars + 20;       // [map] O of an item complete          (commit)
-  uint64_t* o_empty = bars + 22;      // O, maxima and sums read              (128 arrivals)
-  uint64_t* ml_full = bars + 23;      // maxima and sums of an item written   (512 arrivals)
-  uint64_t* drain = bars + 24;        // [4] after an abort: issued MMAs done (commit)
-  uint64_t* m_full = bars + 28;       // [map][parity][quarter] m after a half (32 arrivals)
-  uint64_t* k_full = bars + 44;       // [stage]                              (tx bytes)
-  uint64_t* k_empty = k_full + kS;    // [stage]                              (2 commits)
+  uint64_t* q_empty = bars + 2;       // [2] both maps' S MMAs read it        (commit)
+  uint64_t* s_full = bars + 4;        // [map] S ready                        (commit)
+  uint64_t* p_full = bars + 6;        // [map][part] part of P written        (128 arrivals)
+  uint64_t* pv_done = bars + 10;      // [map] P V done: P consumed           (commit)
+  uint64_t* o_full = bars + 12;       // [map] O of an item complete          (commit)
+  uint64_t* o_empty = bars + 14;      // O, maxima and sums read              (128 arrivals)
+  uint64_t* ml_full = bars + 15;      // maxima and sums of an item written   (256 arrivals)
+  uint64_t* drain = bars + 16;        // after an abort: issued MMAs done     (commit)
+  uint64_t* k_full = bars + 17;       // [stage]                              (tx bytes)
+  uint64_t* k_empty = k_full + kS;    // [stage]                              (commit)
   uint64_t* v_full = k_empty + kS;    // [stage]                              (tx bytes)
-  uint64_t* v_empty = v_full + kS;    // [stage]                              (2 commits)
+  uint64_t* v_empty = v_full + kS;    // [stage]                              (commit)
   uint64_t* v_ready = v_empty + kS;   // [stage] hidden rows cleared          (32 arrivals)
   uint64_t* bits_full = v_ready + kS; // [stage] key mask bits written        (32 arrivals)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bits_full + kS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert((44 + 6 * kS) * 8 + 8 <= G::kBars, "barrier space");
+  static_assert((17 + 6 * kS) * 8 + 8 <= G::kBars, "barrier space");
   float2* ml = reinterpret_cast<float2*>(smem + G::kMlOff);
-  float* m_sh = reinterpret_cast<float*>(smem + G::kMOff);
   uint32_t* mask_bits = reinterpret_cast<uint32_t*>(smem + G::kMaskOff);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1);
-      mbar_init(&q_empty[i], 2);
-      mbar_init(&s_full[2 * i], 1);
-      mbar_init(&s_full[2 * i + 1], 1);
-      for (int j = 0; j < 4; ++j) mbar_init(&p_full[4 * i + j], kTile);
-      mbar_init(&pv_done[2 * i], 1);
-      mbar_init(&pv_done[2 * i + 1], 1);
+      mbar_init(&q_empty[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[2 * i], kTile);
+      mbar_init(&p_full[2 * i + 1], kTile);
+      mbar_init(&pv_done[i], 1);
       mbar_init(&o_full[i], 1);
-      mbar_init(&drain[i], 1);
-      mbar_init(&drain[2 + i], 1);
     }
-    for (int i = 0; i < 16; ++i) mbar_init(&m_full[i], 32);
+    mbar_init(drain, 1);
     mbar_init(o_empty, kTile);
-    mbar_init(ml_full, 4 * kTile);
+    mbar_init(ml_full, 2 * kTile);
     for (int i = 0; i < kS; ++i) {
       mbar_init(&k_full[i], 1);
-      mbar_init(&k_empty[i], 2);
+      mbar_init(&k_empty[i], 1);
       mbar_init(&v_full[i], 1);
-      mbar_init(&v_empty[i], 2);
+      mbar_init(&v_empty[i], 1);
       mbar_init(&v_ready[i], 32);
       mbar_init(&bits_full[i], 32);
     }
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == kScoreWarp) {
+  if (warp == kMmaWarp) {
     tmem_alloc(tmem_slot, kTmemCols);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const bool has_mask = a.key_mask != nullptr;
 
   if (warp < kEpiWarp) {
     // ------------------------------------------------------------ softmax
-    regs_inc<kRegsSoft>();
-    const int map = warp >> 3, group = warp >> 2 & 1, quarter = warp & 3;
+    set_regs<kRegsLaunch, kRegsSoft>();
+    const int map = warp >> 2, quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t s_addr = tmem + lanes + map * 128 + group * kHalf;
     const uint32_t o_addr = tmem + lanes + G::kO + map * G::kDv;
-    float* m_own = m_sh + (map * 2 + group) * kTile + row;
-    const float* m_other = m_sh + (map * 2 + (group ^ 1)) * kTile + row;
-    uint64_t* m_own_full = &m_full[(map * 2 + group) * 4 + quarter];
-    uint64_t* m_other_full = &m_full[(map * 2 + (group ^ 1)) * 4 + quarter];
     const float scale = a.scale_log2;
-    int first_half = 0, first_tile = 0, busy = 0;  // halves, tiles and items with keys before this item
+    const uint32_t s_addr = tmem + lanes + map * 128;
+    int tile = 0, busy = 0;  // tiles and items with keys so far
     bool ok = true;
     for (int round = 0, at; ok && (at = item_at(round)) < items.count; ++round) {
-      int b, h, qt, split, n, u0, u1;
+      int b, h, qt, split, n, t0, t1;
       item_of(a, items, at, b, h, qt, split);
-      halves_of(a, items, b, qt, split, n, u0, u1);
-      if (u0 >= u1) continue;
+      tiles_of(a, items, b, qt, split, n, t0, t1);
+      if (t0 >= t1) continue;
       int lo, hi, common_lo, common_hi, x0, x1;
       const int i0 = qt * kTile, i1 = min(a.d.q_len, i0 + kTile) - 1, i = min(i0 + row, i1);
       key_range_n(a.d, n, i, i, lo, hi);
       key_range_n(a.d, n, i1, i1, common_lo, x1);
       key_range_n(a.d, n, i0, i0, x0, common_hi);
-      float m = -INFINITY, l = 0.0f;  // of this group's halves; l is relative to m
-      for (int u = u0 + ((first_half ^ group) & 1); u < u1; u += 2) {
-        const int half = first_half + u - u0, tile = first_tile + ((u - u0) >> 1), stage = tile % kS;
-        const bool inside = !has_mask && u * kHalf >= common_lo && (u + 1) * kHalf <= common_hi;
-        if (!KB_WARP_WAIT(&s_full[2 * map + group], (half >> 1) & 1) ||
-            (has_mask && !KB_WARP_WAIT(&bits_full[stage], (tile / kS) & 1))) {
+      float m = -INFINITY, l = 0.0f;
+      for (int t = t0; t < t1; ++t, ++tile) {
+        const int stage = tile % kS;
+        if (!KB_WARP_WAIT(&s_full[map], tile & 1) || (has_mask && !KB_WARP_WAIT(&bits_full[stage], (tile / kS) & 1))) {
           ok = false;
           break;
         }
         tc_fence_after();
-        // Scores of 32 keys, hidden ones at -inf.
-        auto load = [&](uint32_t (&s)[32], int c) {
-          tmem_ld32(s_addr + 32 * c, s);
-          tmem_ld_wait(s);
-          if (!inside) {
-            const int base = u * kHalf + 32 * c;
-            uint32_t see = bits_between(lo - base, hi - base);
-            if (has_mask) see &= mask_bits[stage * 4 + (u & 1) * 2 + c];
+        uint32_t s[kTile];
 #pragma unroll
-            for (int k = 0; k < 32; ++k)
-              if (!(see >> k & 1u)) s[k] = 0xff800000u;
-          }
-        };
-        auto maximum = [&](const uint32_t (&s)[32]) -> float {
-          float top[4];
+        for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(s + 32 * c));
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld_wait(*reinterpret_cast<uint32_t(*)[32]>(s + 32 * c));
+        if (has_mask || t * kTile < common_lo || (t + 1) * kTile > common_hi) {  // hidden keys to -inf
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            top[c] = fmaxf(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1]));
+            const int base = t * kTile + 32 * c;
+            uint32_t see = bits_between(lo - base, hi - base);
+            if (has_mask) see &= mask_bits[stage * 4 + c];
 #pragma unroll
-            for (int k = 1; k < 4; ++k)
-              top[c] = max3(top[c], __uint_as_float(s[8 * k + 2 * c]), __uint_as_float(s[8 * k + 2 * c + 1]));
+            for (int k = 0; k < 32; ++k)
+              if (!(see >> k & 1u)) s[32 * c + k] = 0xff800000u;
           }
-          return fmaxf(max3(top[0], top[1], top[2]), top[3]);
-        };
-        uint32_t s[32];
-        load(s, 1);
-        float now = maximum(s);
-        load(s, 0);  // keys 32.. are read again below: registers for both would halve the warps
-        now = fmaxf(now, maximum(s)) * scale;
-
-        // The running maximum of the half before, raised if some row of the
-        // warp is too far above it.
-        if (half > 0 && !KB_WARP_WAIT(m_other_full, ((half - 1) >> 1) & 1)) {
-          ok = false;
-          break;
         }
-        float top = u > u0 ? *m_other : -INFINITY;
-        if (__any_sync(0xffffffffu, now > top + kLazy || (top == -INFINITY && now > -INFINITY))) {
-          const float next = fmaxf(top, now);
-          const float f = top == -INFINITY ? 1.0f : ex2(top - next);  // O is 0 before the first key
-          top = next;
-          if (u > u0) {
-            if (!KB_WARP_WAIT(&pv_done[2 * map + (group ^ 1)], ((half - 1) >> 1) & 1)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
+        float top[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          top[c] = __uint_as_float(s[c]);
+#pragma unroll
+          for (int k = 8 + c; k < kTile - 8; k += 16)
+            top[c] = max3(top[c], __uint_as_float(s[k]), __uint_as_float(s[k + 8]));
+          top[c] = max3(top[c], __uint_as_float(s[kTile - 8 + c]), -INFINITY);
+        }
+        const float now = max3(max3(top[0], top[1], top[2]), max3(top[3], top[4], top[5]), max3(top[6], top[7], -INFINITY)) * scale;
+        // Raise the running maximum if some row of the warp is too far above it.
+        if (__any_sync(0xffffffffu, now > m + kLazy || (m == -INFINITY && now > -INFINITY))) {
+          const float next = fmaxf(m, now);
+          const float f = m == -INFINITY ? 1.0f : ex2(m - next);  // sums are 0 before the first key
+          m = next;
+          l *= f;
+          if (t > t0) {
 #pragma unroll 1
             for (int c = 0; c < static_cast<int>(G::kDv) / 16; ++c) {
               uint32_t o[16];
               tmem_ld16(o_addr + 16 * c, o);
-              tmem_ld_wait();
+              tmem_ld_wait(o);
 #pragma unroll
               for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
               tmem_st16(o_addr + 16 * c, o);
             }
-            tmem_st_wait();
-            tc_fence_before();
           }
         }
-        *m_own = top;
-        mbar_arrive(m_own_full);
-        if (m != top) l *= ex2(m - top);
-        m = top;
 
-        // P of 32 keys at a time: P V of the first starts while the second is at work.
         const float base = m == -INFINITY ? 0.0f : m;
         float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+        // P of 32 keys at a time; P V of the first part starts while the second is at work.
 #pragma unroll
-        for (int part = 0; part < 2; ++part) {
-          if (part) load(s, 1);
+        for (int c = 0; c < 4; ++c) {
           uint32_t pk[16];
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
-            const float2 x = fma2(make_float2(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])),
+            const float2 x = fma2(make_float2(__uint_as_float(s[32 * c + 2 * k]), __uint_as_float(s[32 * c + 2 * k + 1])),
                                   make_float2(scale, scale), make_float2(-base, -base));
             const float2 p = make_float2(ex2(x.x), ex2(x.y));
             sum[k & 1] = add2(sum[k & 1], p);
             pk[k] = pack16x2(p, F16);
           }
-          tmem_st16(s_addr + 16 * part, pk);
-          tmem_st_wait();
-          tc_fence_before();
-          mbar_arrive(&p_full[4 * map + 2 * group + part]);
+          tmem_st16(s_addr + 16 * c, pk);
+          if (32 * (c + 1) == kFirst || c == 3) {
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(&p_full[2 * map + (c == 3)]);
+          }
         }
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       }
       if (!ok) break;
-      first_half += u1 - u0;
-      first_tile += (u1 - u0 + 1) >> 1;
       // The epilogue has read the previous item's maxima and sums.
       if (busy > 0 && !KB_WARP_WAIT(o_empty, (busy - 1) & 1)) break;
-      ml[(map * 2 + group) * kTile + row] = make_float2(m, l);
+      ml[map * kTile + row] = make_float2(m, l);
       mbar_arrive(ml_full);
       ++busy;
     }
-  } else if (warp < kScoreWarp) {
+  } else if (warp < kMmaWarp) {
     // ------------------------------------------------------------ epilogue
+    set_regs<kRegsLaunch, kRegsEpi>();
     const int row = threadIdx.x & (kTile - 1);
     const uint32_t o_addr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + G::kO;
     int busy = 0;
     for (int round = 0, at; (at = item_at(round)) < items.count; ++round) {
-      int b, h, qt, split, n, u0, u1;
+      int b, h, qt, split, n, t0, t1;
       item_of(a, items, at, b, h, qt, split);
-      halves_of(a, items, b, qt, split, n, u0, u1);
+      tiles_of(a, items, b, qt, split, n, t0, t1);
       const int i = qt * kTile + row;
       const bool live = i < a.d.q_len;
-      const bool any = u0 < u1;
+      const bool any = t0 < t1;
       float2 v0 = make_float2(-INFINITY, 0.0f), v1 = v0;
       if (any) {
         if (!KB_WARP_WAIT(ml_full, busy & 1) || !KB_WARP_WAIT(&o_full[0], busy & 1) ||
             !KB_WARP_WAIT(&o_full[1], busy & 1))
           break;
         tc_fence_after();
-        v0 = joined(ml[row], ml[kTile + row]);
-        v1 = joined(ml[2 * kTile + row], ml[3 * kTile + row]);
+        v0 = ml[row], v1 = ml[kTile + row];
       }
       if (items.splits > 1) {
         const int64_t at2 = live ? (row_index(a, b, i, h) * items.splits + split) * 2 : 0;
@@ -498,70 +470,81 @@ __global__ void __launch_bounds__(kThreads, 1) diff_tc_kernel(const __grid_const
       }
     }
   } else {
-    regs_dec<kRegsRest>();
+    set_regs<kRegsLaunch, kRegsRest>();
     constexpr uint32_t kFmt = F16 ? 0u : 1u;
     constexpr uint32_t kId = (1u << 4) | (kFmt << 7) | (kFmt << 10) | (static_cast<uint32_t>(128 >> 4) << 24);
-    constexpr uint32_t kIdS = kId | (static_cast<uint32_t>(kHalf >> 3) << 17);
+    constexpr uint32_t kIdS = kId | (static_cast<uint32_t>(kTile >> 3) << 17);
     constexpr uint32_t kIdV = kId | (1u << 16) /* B MN-major */ | (G::kDv >> 3 << 17);
-    constexpr uint32_t kHalfRows = kHalf * D * 2, kHalfV = kHalf * 128;  // bytes to the second half of a tile
-    if (warp < kValueWarp) {
-      // ---------------------------------------------------------- S of one map
-      if (lane == 0) {
-        const int map = warp - kScoreWarp;
-        Walk w;
-        w.start(a, items);
-        bool ok = true;
-        for (int i = 0; ok && w.valid; ++i) {  // i counts halves
-          const int stage = w.tile % kS;
-          ok = (w.u > w.u0 || mbar_wait(&q_full[w.item & 1], (w.item >> 1) & 1, abort_flag)) &&
-               mbar_wait(&k_full[stage], (w.tile / kS) & 1, abort_flag);
-          const uint64_t qdesc = tile_desc<D>(smem_u32(smem + G::kQOff + ((w.item & 1) * 2 + map) * G::kQk));
-          const uint64_t kdesc =
-              tile_desc<D>(smem_u32(smem + G::kKOff + (stage * 2 + map) * G::kQk + (w.u & 1) * kHalfRows));
-          // It overwrites the P of the half before last.
-          ok = ok && (i < 2 || mbar_wait(&pv_done[2 * map + (i & 1)], ((i >> 1) - 1) & 1, abort_flag));
-          if (!ok) break;
-          tc_fence_after();
+    if (warp == kMmaWarp) {
+      // ---------------------------------------------------------- MMA issue
+      // The whole warp walks and waits; one lane issues.
+      Walk ws, wp;  // the tiles whose S and whose P V come next
+      ws.start(a, items);
+      wp = ws;
+      auto issue_s = [&](int map) -> bool {
+        const int stage = ws.tile % kS;
+        if (map == 0 && ((ws.begins_item() && !KB_WARP_WAIT(&q_full[ws.item & 1], (ws.item >> 1) & 1)) ||
+                         !KB_WARP_WAIT(&k_full[stage], (ws.tile / kS) & 1)))
+          return false;
+        const uint64_t qdesc = tile_desc<D>(smem_u32(smem + G::kQOff + ((ws.item & 1) * 2 + map) * G::kQk));
+        const uint64_t kdesc = tile_desc<D>(smem_u32(smem + G::kKOff + (stage * 2 + map) * G::kQk));
+        // It overwrites the P of the tile before.
+        if (ws.tile > 0 && !KB_WARP_WAIT(&pv_done[map], (ws.tile - 1) & 1)) return false;
+        tc_fence_after();
+        if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < D / 16; ++k)
-            mma_issue<kKindBF16>(tmem + map * 128 + (i & 1) * kHalf, qdesc + 2 * k, kdesc + 2 * k, kIdS, k != 0, 0, 0);
-          tc_commit(&s_full[2 * map + (i & 1)]);
-          if (w.ends_tile()) tc_commit(&k_empty[stage]);
-          if (w.ends_item()) tc_commit(&q_empty[w.item & 1]);
-          w.step(a, items);
-        }
-        drain_mmas(&drain[map], abort_flag);
-      }
-    } else if (warp < kLoadWarp) {
-      // ---------------------------------------------------------- P V of one map
-      if (lane == 0) {
-        const int map = warp - kValueWarp;
-        const uint32_t o_tmem = tmem + G::kO + map * G::kDv;
-        Walk w;
-        w.start(a, items);
-        bool ok = true;
-        for (int i = 0; ok && w.valid; ++i) {
-          const int stage = w.tile % kS, buf = i & 1;
-          const uint64_t vdesc =
-              sw128_mn_desc(smem_u32(smem + G::kVOff + stage * G::kV + (w.u & 1) * kHalfV), G::kVCol);
-          ok = mbar_wait(&v_ready[stage], (w.tile / kS) & 1, abort_flag) &&
-               (w.u > w.u0 || w.item == 0 || mbar_wait(o_empty, (w.item - 1) & 1, abort_flag));
-          for (int part = 0; part < 2 && ok; ++part) {
-            ok = mbar_wait(&p_full[4 * map + 2 * buf + part], (i >> 1) & 1, abort_flag);
-            if (!ok) break;
-            tc_fence_after();
-#pragma unroll
-            for (int k = 2 * part; k < 2 * part + 2; ++k)
-              mma_f16_ts(o_tmem, tmem + map * 128 + buf * kHalf + 8 * k,
-                         vdesc + static_cast<uint64_t>(k * 16 * 128 >> 4), kIdV, w.u > w.u0 || k != 0);
+            mma_issue<kKindBF16>(tmem + map * 128, qdesc + 2 * k, kdesc + 2 * k, kIdS, k != 0, 0, 0);
+          tc_commit(&s_full[map]);
+          if (map == 1) {
+            tc_commit(&k_empty[stage]);
+            if (ws.ends_item()) tc_commit(&q_empty[ws.item & 1]);
           }
-          if (!ok) break;
-          tc_commit(&pv_done[2 * map + buf]);
-          if (w.ends_tile()) tc_commit(&v_empty[stage]);
-          if (w.ends_item()) tc_commit(&o_full[map]);
-          w.step(a, items);
         }
-        drain_mmas(&drain[2 + map], abort_flag);
+        __syncwarp();
+        if (map == 1) ws.step(a, items);
+        return true;
+      };
+      auto issue_pv = [&](int map) -> bool {
+        const int stage = wp.tile % kS;
+        const uint64_t vdesc = sw128_mn_desc(smem_u32(smem + G::kVOff + stage * G::kV), G::kVCol);
+        if (map == 0 && (!KB_WARP_WAIT(&v_ready[stage], (wp.tile / kS) & 1) ||
+                         (wp.begins_item() && wp.item > 0 && !KB_WARP_WAIT(o_empty, (wp.item - 1) & 1))))
+          return false;
+        const uint32_t add = !wp.begins_item();
+        if (!KB_WARP_WAIT(&p_full[2 * map], wp.tile & 1)) return false;
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < kFirst / 16; ++k)
+            mma_f16_ts(tmem + G::kO + map * G::kDv, tmem + map * 128 + 8 * k,
+                       vdesc + static_cast<uint64_t>(k * 16 * 128 >> 4), kIdV, k == 0 ? add : 1u);
+        }
+        __syncwarp();
+        if (!KB_WARP_WAIT(&p_full[2 * map + 1], wp.tile & 1)) return false;
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int k = kFirst / 16; k < kTile / 16; ++k)
+            mma_f16_ts(tmem + G::kO + map * G::kDv, tmem + map * 128 + 8 * k,
+                       vdesc + static_cast<uint64_t>(k * 16 * 128 >> 4), kIdV, 1u);
+          tc_commit(&pv_done[map]);
+          if (wp.ends_item()) tc_commit(&o_full[map]);
+          if (map == 1) tc_commit(&v_empty[stage]);
+        }
+        __syncwarp();
+        if (map == 1) wp.step(a, items);
+        return true;
+      };
+      bool ok = !ws.valid || (issue_s(0) && issue_s(1));
+      while (ok && wp.valid) {
+        const bool more = ws.valid;
+        ok = issue_pv(0) && (!more || issue_s(0)) && issue_pv(1) && (!more || issue_s(1));
+      }
+      if (__any_sync(0xffffffffu, *abort_flag) && elect_one()) {
+        int none = 0;  // let the MMAs issued so far finish before tensor memory goes
+        tc_commit(drain);
+        mbar_wait(drain, 0, &none);
       }
     } else if (warp == kLoadWarp) {
       // ---------------------------------------------------------- TMA loads
@@ -573,13 +556,12 @@ __global__ void __launch_bounds__(kThreads, 1) diff_tc_kernel(const __grid_const
         int tile = 0, tile_v = 0, busy = 0;  // K tiles, V tiles and items loaded
         bool ok = true;
         for (int round = 0, at; ok && (at = item_at(round)) < items.count; ++round) {
-          int b, h, qt, split, n, u0, u1;
+          int b, h, qt, split, n, t0, t1;
           item_of(a, items, at, b, h, qt, split);
-          halves_of(a, items, b, qt, split, n, u0, u1);
-          if (u0 >= u1) continue;
-          const int t0 = u0 / 2, t1 = (u1 + 1) / 2;
+          tiles_of(a, items, b, qt, split, n, t0, t1);
+          if (t0 >= t1) continue;
           const int hk = h / share, qb = busy & 1;
-          ok = mbar_wait(&q_empty[qb], ((busy >> 1) & 1) ^ 1, abort_flag);
+          ok = wait_short(&q_empty[qb], ((busy >> 1) & 1) ^ 1, abort_flag);
           if (!ok) break;
           mbar_arrive_expect_tx(&q_full[qb], 2 * G::kQk);
           for (int m = 0; m < 2; ++m)
@@ -589,14 +571,14 @@ __global__ void __launch_bounds__(kThreads, 1) diff_tc_kernel(const __grid_const
           for (int t = t0; t < t1; ++t) {
             const int stage = tile % kS;
             const uint32_t parity = ((tile / kS) & 1) ^ 1;
-            ok = mbar_wait(&k_empty[stage], parity, abort_flag);
+            ok = wait_short(&k_empty[stage], parity, abort_flag);
             if (!ok) break;
             mbar_arrive_expect_tx(&k_full[stage], 2 * G::kQk);
             for (int m = 0; m < 2; ++m)
               tma_load_5d(smem + G::kKOff + (stage * 2 + m) * G::kQk, &map_k, &k_full[stage], 0, t * kTile,
                           hk * bc.k_head, m * bc.k_map, b * bc.k_batch);
             ++tile;
-            ok = mbar_wait(&v_empty[stage], parity, abort_flag);
+            ok = wait_short(&v_empty[stage], parity, abort_flag);
             if (!ok) break;
             mbar_arrive_expect_tx(&v_full[stage], G::kV);
             for (int c = 0; c < static_cast<int>(G::kDv) / 64; ++c)
@@ -617,10 +599,9 @@ __global__ void __launch_bounds__(kThreads, 1) diff_tc_kernel(const __grid_const
       int tile = 0;
       bool ok = true;
       for (int round = 0, at; ok && (at = item_at(round)) < items.count; ++round) {
-        int b, h, qt, split, n, u0, u1;
+        int b, h, qt, split, n, t0, t1;
         item_of(a, items, at, b, h, qt, split);
-        halves_of(a, items, b, qt, split, n, u0, u1);
-        const int t0 = u0 / 2, t1 = (u1 + 1) / 2;
+        tiles_of(a, items, b, qt, split, n, t0, t1);
         const uint8_t* mask = has_mask ? a.key_mask + b * a.d.mask_batch : nullptr;
         for (int t = t0; t < t1; ++t, ++tile) {
           const int stage = tile % kS;
@@ -665,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, 1) diff_tc_kernel(const __grid_const
   __syncthreads();
   tc_fence_after();
   if (threadIdx.x == 0 && *abort_flag) record_status(status, KB_STATUS_TIMEOUT, KB_NO_LAYER);
-  if (warp == kScoreWarp) tmem_dealloc(tmem, kTmemCols);
+  if (warp == kMmaWarp) tmem_dealloc(tmem, kTmemCols);
 }
 
 #undef KB_WARP_WAIT
@@ -700,8 +681,8 @@ int launch(const DiffArgs& a, int splits, unsigned* status, cudaStream_t s) {
     cudaFuncAttributes attr;
     int rc = check_cuda(cudaFuncGetAttributes(&attr, kern), "differential attention attributes");
     if (rc) return rc;
-    if (attr.numRegs * kThreads < 128 * (4 * kRegsSoft + kRegsEpi + 2 * kRegsRest)) {
-      set_error("differential attention: the kernel was built with too few registers for its split");
+    if (attr.numRegs != kRegsLaunch) {
+      set_error("differential attention: the kernel was not built with the registers of its split");
       return KB_E_UNSUPPORTED;
     }
     rc = smem_opt_in(reinterpret_cast<const void*>(kern), Geo<D>::kBytes);

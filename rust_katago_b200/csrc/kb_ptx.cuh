@@ -43,6 +43,21 @@ __device__ __forceinline__ uint64_t globaltimer() {
   return t;
 }
 
+// True in one lane of a converged warp.  Unlike a test of the lane number it
+// tells the compiler that the branch is warp-uniform, so the operands of the
+// tensor-core instructions behind it stay in uniform registers: with them in
+// per-thread registers one thread issued an MMA every 95 clocks (of 64 that it
+// takes).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+
 __device__ __forceinline__ uint32_t elect_lane0() { return (threadIdx.x & 31) == 0; }
 
 // ---------------------------------------------------------------- mbarrier
@@ -420,12 +435,15 @@ __device__ __forceinline__ void tmem_st1(uint32_t taddr, uint32_t r) {
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Move registers between the warpgroups of a block; every warp of a warpgroup
-// executes the same one.  The groups' shares must not exceed the launch's total.
-template <int N>
-__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N>
-__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+// Set this warpgroup's registers per thread to N from the LAUNCH per thread
+// that the block was launched with.  Every warpgroup of the block calls it, all
+// warps of one with the same N; an increase waits until the others have given
+// up enough, for ever if the shares add up to more than the launch's.
+template <int LAUNCH, int N>
+__device__ __forceinline__ void set_regs() {
+  if constexpr (N > LAUNCH) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+  if constexpr (N < LAUNCH) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 
 // Record an error in a sticky status word [flags, first_layer]: flags are OR-ed,
 // the first reporting layer wins.
