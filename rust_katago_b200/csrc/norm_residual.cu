@@ -1,12 +1,23 @@
 // The norms around a block in one pass (kb_norm_residual):
 //   r = res_scale * x + branch_scale * act(gate) * post_norm(y)
 //   h = pre_norm(r) * (1 + mod_scale) + mod_shift
-// x and y are read once, r and h written once, so HBM bounds it.  A group of
-// threads (one warp, or one block for wide rows) holds a row in registers as
-// fp32 from the first load to the last store; both norms reduce over the
-// group.  Variances are taken from the centred values, not as E[v^2] - E[v]^2.
-// h is computed from the unrounded r: rounding r first would add its error to h.
+// x and y are read once, r and h written once, so HBM bounds it.
+//
+// A group of threads (one warp, or one block for wide rows) walks a run of
+// neighbouring rows and holds a row in registers as fp32 from the first load to
+// the last store; the next row's x and y are loaded while this one is at work.
+// What rows share is folded into at most four vectors in registers, built
+// again only when the row of gate and modulation changes:
+//   r = res_scale x + G n' + C   G = branch_scale gate gamma, C = branch_scale gate beta
+//   h = A r' + B                 A = gamma' (1 + mod_scale),  B = beta' (1 + mod_scale) + mod_shift
+// with n' and r' the normalised values.  (With the vectors applied one by one
+// and the types chosen at run time, the instructions bounded it: 92,416 x 768
+// took 317 us.)  Variances are taken from the centred values, not as E[v^2] -
+// E[v]^2.  h is computed from the unrounded r: rounding r first would add its
+// error to h.
 #include <stdint.h>
+
+#include <atomic>
 
 #include "kb_internal.h"
 #include "kb_numeric.cuh"
@@ -22,88 +33,369 @@ struct NormArgs {
   void *x_out, *h;
 };
 
-// Values of one row held by one thread: NC chunks of 8.  VEC: chunk c holds
-// columns 8 (c TPR + i) .. + 7 (16- or 32-byte accesses); otherwise element e
-// of chunk c is column (8 c + e) TPR + i, one element per access.
-template <int NC, bool VEC>
-__device__ __forceinline__ int column(int c, int e, int i, int tpr) {
-  return VEC ? (c * tpr + i) * 8 + e : (c * 8 + e) * tpr + i;
+// Runs of rows per resident group: a few, so that groups that finish early
+// leave little idle.
+constexpr int kRunsPerSlot = 2;
+// ------------------------------------------------------------------ whole groups of eight columns
+// Eight columns of type DT as fp32 pairs, and back.
+template <int DT>
+struct Raw8 {
+  uint4 w[DT == KB_DT_F32 ? 2 : 1];
+};
+
+template <int DT>
+__device__ __forceinline__ Raw8<DT> load8(const void* p, int64_t at) {
+  Raw8<DT> r;
+  const uint4* q = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) + at * (DT == KB_DT_F32 ? 4 : 2));
+  r.w[0] = __ldg(q);
+  if constexpr (DT == KB_DT_F32) r.w[1] = __ldg(q + 1);
+  return r;
 }
 
-__device__ __forceinline__ void unpack8(const uint4& w, bool f16, float* v) {
-  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+template <int DT>
+__device__ __forceinline__ void open8(const Raw8<DT>& r, float2 (&v)[4]) {
+  const uint32_t u[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    v[2 * i] = from16(static_cast<uint16_t>(u[i] & 0xffffu), f16);
-    v[2 * i + 1] = from16(static_cast<uint16_t>(u[i] >> 16), f16);
+    if constexpr (DT == KB_DT_F32) {
+      const uint4& w = r.w[i >> 1];
+      v[i] = i & 1 ? make_float2(__uint_as_float(w.z), __uint_as_float(w.w))
+                   : make_float2(__uint_as_float(w.x), __uint_as_float(w.y));
+    } else if constexpr (DT == KB_DT_F16) {
+      v[i] = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+    } else {
+      v[i] = make_float2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
+    }
   }
 }
 
-// Load the row piece of type `dtype` (KB_DT_*, uniform) at p.
-template <int NC, bool VEC>
-__device__ __forceinline__ void load_row(const void* p, int64_t offset, int dtype, int width, int i, int tpr,
-                                         float (&v)[NC * 8]) {
+template <int DT>
+__device__ __forceinline__ void store8(void* p, int64_t at, const float2 (&v)[4]) {
+  if constexpr (DT == KB_DT_F32) {
+    float4* q = reinterpret_cast<float4*>(static_cast<float*>(p) + at);
+    q[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+    q[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+  } else {
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + at) =
+        make_uint4(pack16x2(v[0], DT == KB_DT_F16), pack16x2(v[1], DT == KB_DT_F16), pack16x2(v[2], DT == KB_DT_F16),
+                   pack16x2(v[3], DT == KB_DT_F16));
+  }
+}
+
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// Sum of v over the row's threads.  BLOCK: `red` holds two sets of one float
+// per warp (zeros past the last) that successive sums alternate between, so
+// each needs one barrier.
+template <bool BLOCK>
+__device__ __forceinline__ float group_sum(float2 v, float (*red)[16], int& turn) {
+  float s = v.x + v.y;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if constexpr (BLOCK) {
+    float* slot = red[turn];
+    turn ^= 1;
+    if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = s;
+    __syncthreads();
+    const float4* q = reinterpret_cast<const float4*>(slot);
+    const float4 a = q[0], b = q[1], c = q[2], d = q[3];
+    s = ((a.x + a.y) + (a.z + a.w)) + ((b.x + b.y) + (b.z + b.w)) + (((c.x + c.y) + (c.z + c.w)) + ((d.x + d.y) + (d.z + d.w)));
+  }
+  return s;
+}
+
+// v -> v centred (KB_NORM_LAYER); returns the factor 1 / sqrt(mean(v^2) + eps),
+// or 1 without a norm.  Chunks outside the row hold zeros.
+template <int NC, bool BLOCK>
+__device__ __forceinline__ float normalise(float2 (&v)[NC][4], int kind, float inv_width, float eps, int valid,
+                                           float (*red)[16], int& turn) {
+  if (kind == KB_NORM_NONE) return 1.0f;
+  if (kind == KB_NORM_LAYER) {
+    float2 s = both(0.0f);
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s = add2(s, v[c][i]);
+    const float mean = group_sum<BLOCK>(s, red, turn) * inv_width;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      if (c < valid)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[c][i] = add2(v[c][i], both(-mean));
+  }
+  float2 s0 = both(0.0f), s1 = both(0.0f);
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+      s0 = fma2(v[c][i], v[c][i], s0);
+      s1 = fma2(v[c][i + 1], v[c][i + 1], s1);
+    }
+  return rsqrtf(group_sum<BLOCK>(add2(s0, s1), red, turn) * inv_width + eps);
+}
+
+__device__ __forceinline__ float gate_value(float v, int act) {
+  if (act == KB_GATE_SIGMOID) return 1.0f / (1.0f + expf(-v));
+  if (act == KB_GATE_TANH) return tanhf(v);
+  return v;
+}
+
+// XT, YT: types of stream and branch.  SHIFT: 0 no shifts, 1 only B, 2 also C.
+// THREADS: 32 (a warp per row, the vectors in registers) or the most that a
+// block has (the vectors in shared memory, each thread's own columns).
+template <int XT, int YT, int NC, int THREADS, int SHIFT>
+__global__ void __launch_bounds__(THREADS, THREADS == 320 ? 2 : 1) norm_rows_kernel(const NormArgs a,
+                                                                                   int rows_per_group) {
+  constexpr bool BLOCK = THREADS > 32;
+  __shared__ alignas(16) float red[2][16];
+  extern __shared__ float4 shared_vectors[];  // [vector][chunk][half][thread]
+  if constexpr (BLOCK) {
+    if (threadIdx.x < 32) reinterpret_cast<float*>(red)[threadIdx.x] = 0.0f;
+    __syncthreads();
+  }
+  const kb_norm_residual_desc& d = a.d;
+  const int tpr = BLOCK ? blockDim.x : 32;
+  const int i = threadIdx.x;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * rows_per_group;
+  const int64_t end = min(row + rows_per_group, static_cast<int64_t>(d.rows));
+  if (row >= end) return;
+  const int col = i * 8, step = tpr * 8;
+  int valid = 0;  // chunks of this thread inside the row
+#pragma unroll
+  for (int c = 0; c < NC; ++c) valid += col + c * step < d.width;
+  const float inv_width = 1.0f / static_cast<float>(d.width);
+  int turn = 0;
+
+  // The vectors G, A, B, C: chunk c of this thread.
+  constexpr int kHeld = BLOCK ? 1 : NC;
+  float2 held[4][kHeld][4];
+  auto keep = [&](int which, int c, const float2 (&v)[4]) {
+    if constexpr (BLOCK) {
+      float4* at = shared_vectors + (which * NC + c) * 2 * tpr + i;
+      at[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+      at[tpr] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) held[which][c][k] = v[k];
+    }
+  };
+  auto vector = [&](int which, int c, float2 (&v)[4]) {
+    if constexpr (BLOCK) {
+      const float4* at = shared_vectors + (which * NC + c) * 2 * tpr + i;
+      const float4 p = at[0], q = at[tpr];
+      v[0] = make_float2(p.x, p.y), v[1] = make_float2(p.z, p.w), v[2] = make_float2(q.x, q.y), v[3] = make_float2(q.z, q.w);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = held[which][c][k];
+    }
+  };
+  auto vectors = [&](int64_t cond) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      float2 gv[4], av[4], cv[4], bv[4];
+      const int at = col + c * step;
+      float2 t[4], u[4];
+      const bool in = c < valid;
+      auto param = [&](const float* p, float otherwise, float2 (&v)[4]) {
+        if (p && in) open8<KB_DT_F32>(load8<KB_DT_F32>(p, at), v);
+        else
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[k] = both(otherwise);
+      };
+      auto mod = [&](const void* p, float otherwise, float2 (&v)[4]) {
+        if (p && in) open8<YT>(load8<YT>(p, cond * d.cond_stride + at), v);
+        else
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[k] = both(otherwise);
+      };
+      mod(a.gate, 1.0f, t);
+      param(d.post_norm == KB_NORM_NONE ? nullptr : a.post_gamma, 1.0f, gv);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (a.gate) t[k] = make_float2(gate_value(t[k].x, d.gate_act), gate_value(t[k].y, d.gate_act));
+        t[k] = mul2(t[k], both(d.branch_scale));
+        gv[k] = mul2(gv[k], t[k]);
+      }
+      if constexpr (SHIFT == 2) {
+        param(d.post_norm == KB_NORM_NONE ? nullptr : a.post_beta, 0.0f, u);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) cv[k] = mul2(u[k], t[k]);
+      }
+      mod(a.mod_scale, 0.0f, t);
+      param(d.pre_norm == KB_NORM_NONE ? nullptr : a.pre_gamma, 1.0f, av);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        t[k] = add2(t[k], both(1.0f));
+        av[k] = mul2(av[k], t[k]);
+      }
+      if constexpr (SHIFT) {
+        param(d.pre_norm == KB_NORM_NONE ? nullptr : a.pre_beta, 0.0f, u);
+        mod(a.mod_shift, 0.0f, bv);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) bv[k] = fma2(u[k], t[k], bv[k]);
+        keep(2, c, bv);
+      }
+      keep(0, c, gv);
+      keep(1, c, av);
+      if constexpr (SHIFT == 2) keep(3, c, cv);
+    }
+  };
+
+  Raw8<XT> xr[NC];
+  Raw8<YT> yr[NC];
+  auto fetch = [&](int64_t at) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      if (c >= valid) continue;
+      xr[c] = load8<XT>(a.x, at * d.x_stride + col + c * step);
+      if (a.y) yr[c] = load8<YT>(a.y, at * d.y_stride + col + c * step);
+    }
+  };
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    if constexpr (VEC) {
-      const int col = (c * tpr + i) * 8;
+    xr[c] = Raw8<XT>{};
+    yr[c] = Raw8<YT>{};
+  }
+  fetch(row);
+  const bool conditioned = a.gate || a.mod_scale || a.mod_shift;
+  int64_t cond = conditioned ? row / d.rows_per_cond : 0, next_cond = conditioned ? (cond + 1) * d.rows_per_cond : end;
+  vectors(cond);
+  for (; row < end; ++row) {
+    if (row == next_cond) {
+      vectors(++cond);
+      next_cond += d.rows_per_cond;
+    }
+    float2 r[NC][4], n[NC][4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[c * 8 + e] = 0.0f;
-      if (col < width) {
-        if (dtype == KB_DT_F32) {
-          const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + offset + col);
-          *reinterpret_cast<float4*>(&v[c * 8]) = q[0];
-          *reinterpret_cast<float4*>(&v[c * 8 + 4]) = q[1];
-        } else {
-          unpack8(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + offset + col), dtype == KB_DT_F16,
-                  &v[c * 8]);
+    for (int c = 0; c < NC; ++c) {
+      open8<XT>(xr[c], r[c]);
+      open8<YT>(yr[c], n[c]);
+    }
+    if (row + 1 < end) fetch(row + 1);
+    if (a.y) {
+      const float2 f = both(normalise<NC, BLOCK>(n, d.post_norm, inv_width, d.eps, valid, red, turn));
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        float2 gv[4], cv[4];
+        vector(0, c, gv);
+        if constexpr (SHIFT == 2) vector(3, c, cv);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float2 t = mul2(n[c][k], f);
+          if constexpr (SHIFT == 2) t = fma2(t, gv[k], cv[k]);
+          else t = mul2(t, gv[k]);
+          r[c][k] = fma2(r[c][k], both(d.res_scale), t);
         }
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int col = (c * 8 + e) * tpr + i;
-        v[c * 8 + e] = 0.0f;
-        if (col < width) {
-          if (dtype == KB_DT_F32) v[c * 8 + e] = static_cast<const float*>(p)[offset + col];
-          else v[c * 8 + e] = from16(static_cast<const uint16_t*>(p)[offset + col], dtype == KB_DT_F16);
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) r[c][k] = mul2(r[c][k], both(d.res_scale));
+    }
+    if (a.x_out)
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        if (c < valid) store8<XT>(a.x_out, row * d.x_out_stride + col + c * step, r[c]);
+    if (a.h) {
+      const float2 f = both(normalise<NC, BLOCK>(r, d.pre_norm, inv_width, d.eps, valid, red, turn));
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        if (c >= valid) continue;
+        float2 av[4], bv[4];
+        vector(1, c, av);
+        if constexpr (SHIFT) vector(2, c, bv);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 t = mul2(r[c][k], f);
+          if constexpr (SHIFT) r[c][k] = fma2(t, av[k], bv[k]);
+          else r[c][k] = mul2(t, av[k]);
         }
+        store8<YT>(a.h, row * d.h_stride + col + c * step, r[c]);
       }
     }
   }
 }
 
-template <int NC, bool VEC>
+// Rows of up to 1,024 columns take a warp each (and a block of its own: at 150
+// to 200 registers a thread more warps fit so), wider ones a block of threads
+// with 16 columns each; enough groups to fill the SMs, each with a run of
+// neighbouring rows.
+template <int XT, int YT, int NC, int THREADS, int SHIFT>
+int launch_shift(const NormArgs& a, cudaStream_t s) {
+  auto kern = norm_rows_kernel<XT, YT, NC, THREADS, SHIFT>;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  int threads = 32, bytes = 0, resident = 12;
+  if (THREADS > 32) {
+    threads = (a.d.width / 8 + NC * 32 - 1) / (NC * 32) * 32;
+    bytes = (2 + SHIFT) * NC * threads * 32;
+    resident = THREADS == 320 ? 2 : 1;
+    if (bytes > 48 * 1024) {
+      static std::atomic<uint64_t> configured{0};
+      const uint64_t bit = 1ull << (dev & 63);
+      if (!(configured.load() & bit)) {
+        const int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                       (2 + SHIFT) * NC * THREADS * 32), "norm smem attribute");
+        if (rc) return rc;
+        configured.fetch_or(bit);
+      }
+    }
+  }
+  int64_t groups = static_cast<int64_t>(num_sms(dev)) * kRunsPerSlot * resident;
+  const int64_t per = (a.d.rows + groups - 1) / groups;
+  groups = (a.d.rows + per - 1) / per;
+  kern<<<static_cast<unsigned>(groups), threads, bytes, s>>>(a, static_cast<int>(per));
+  return check_cuda(cudaGetLastError(), "norm launch");
+}
+
+template <int XT, int YT, int NC, int THREADS>
+int launch_rows(const NormArgs& a, cudaStream_t s) {
+  if (a.post_beta) return launch_shift<XT, YT, NC, THREADS, 2>(a, s);
+  if (a.pre_beta || a.mod_shift) return launch_shift<XT, YT, NC, THREADS, 1>(a, s);
+  return launch_shift<XT, YT, NC, THREADS, 0>(a, s);
+}
+
+constexpr int kTypedWidth = 8192;  // the widest row of the typed kernels
+
+template <int XT, int YT>
+int launch_typed(const NormArgs& a, cudaStream_t s) {
+  const int chunks = a.d.width / 8;
+  if (chunks <= 32) return launch_rows<XT, YT, 1, 32>(a, s);
+  if (chunks <= 64) return launch_rows<XT, YT, 2, 32>(a, s);
+  if (chunks <= 96) return launch_rows<XT, YT, 3, 32>(a, s);
+  if (chunks <= 128) return launch_rows<XT, YT, 4, 32>(a, s);
+  if (chunks <= 640) return launch_rows<XT, YT, 2, 320>(a, s);
+  return launch_rows<XT, YT, 2, 512>(a, s);
+}
+
+// ------------------------------------------------------------------ any width and alignment
+// Values of one row held by one thread: element k is column k TPR + i, one
+// element per access, types chosen at run time.
+
+template <int N>
+__device__ __forceinline__ void load_row(const void* p, int64_t offset, int dtype, int width, int i, int tpr,
+                                         float (&v)[N]) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int col = k * tpr + i;
+    v[k] = 0.0f;
+    if (col < width) {
+      if (dtype == KB_DT_F32) v[k] = static_cast<const float*>(p)[offset + col];
+      else v[k] = from16(static_cast<const uint16_t*>(p)[offset + col], dtype == KB_DT_F16);
+    }
+  }
+}
+
+template <int N>
 __device__ __forceinline__ void store_row(void* p, int64_t offset, int dtype, int width, int i, int tpr,
-                                          const float (&v)[NC * 8]) {
+                                          const float (&v)[N]) {
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    if constexpr (VEC) {
-      const int col = (c * tpr + i) * 8;
-      if (col < width) {
-        if (dtype == KB_DT_F32) {
-          float4* q = reinterpret_cast<float4*>(static_cast<float*>(p) + offset + col);
-          q[0] = make_float4(v[c * 8], v[c * 8 + 1], v[c * 8 + 2], v[c * 8 + 3]);
-          q[1] = make_float4(v[c * 8 + 4], v[c * 8 + 5], v[c * 8 + 6], v[c * 8 + 7]);
-        } else {
-          const bool f16 = dtype == KB_DT_F16;
-          uint4 w;
-          w.x = pack16x2(make_float2(v[c * 8], v[c * 8 + 1]), f16);
-          w.y = pack16x2(make_float2(v[c * 8 + 2], v[c * 8 + 3]), f16);
-          w.z = pack16x2(make_float2(v[c * 8 + 4], v[c * 8 + 5]), f16);
-          w.w = pack16x2(make_float2(v[c * 8 + 6], v[c * 8 + 7]), f16);
-          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + offset + col) = w;
-        }
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int col = (c * 8 + e) * tpr + i;
-        if (col < width) {
-          if (dtype == KB_DT_F32) static_cast<float*>(p)[offset + col] = v[c * 8 + e];
-          else static_cast<uint16_t*>(p)[offset + col] = bits16(v[c * 8 + e], dtype == KB_DT_F16);
-        }
-      }
+  for (int k = 0; k < N; ++k) {
+    const int col = k * tpr + i;
+    if (col < width) {
+      if (dtype == KB_DT_F32) static_cast<float*>(p)[offset + col] = v[k];
+      else static_cast<uint16_t*>(p)[offset + col] = bits16(v[k], dtype == KB_DT_F16);
     }
   }
 }
@@ -126,39 +418,36 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
 }
 
 // v = norm(v) * gamma + beta over the row; columns past `width` hold zeros.
-template <int NC, bool VEC, bool BLOCK>
-__device__ __forceinline__ void norm_row(float (&v)[NC * 8], int kind, const float* gamma, const float* beta, float eps,
+template <int N, bool BLOCK>
+__device__ __forceinline__ void norm_row(float (&v)[N], int kind, const float* gamma, const float* beta, float eps,
                                          int width, int i, int tpr, float* red) {
   if (kind == KB_NORM_NONE) return;
   float mean = 0.0f;
   if (kind == KB_NORM_LAYER) {
     float s = 0.0f;
 #pragma unroll
-    for (int k = 0; k < NC * 8; ++k) s += v[k];
+    for (int k = 0; k < N; ++k) s += v[k];
     mean = row_sum<BLOCK>(s, red) / static_cast<float>(width);
   }
   float s = 0.0f;
 #pragma unroll
-  for (int c = 0; c < NC; ++c)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float t = column<NC, VEC>(c, e, i, tpr) < width ? v[c * 8 + e] - mean : 0.0f;
-      v[c * 8 + e] = t;
-      s = fmaf(t, t, s);
-    }
+  for (int k = 0; k < N; ++k) {
+    v[k] = k * tpr + i < width ? v[k] - mean : 0.0f;
+    s = fmaf(v[k], v[k], s);
+  }
   const float rstd = 1.0f / sqrtf(row_sum<BLOCK>(s, red) / static_cast<float>(width) + eps);
-  float g[NC * 8];
-  if (gamma) load_row<NC, VEC>(gamma, 0, KB_DT_F32, width, i, tpr, g);
+  float g[N];
+  if (gamma) load_row(gamma, 0, KB_DT_F32, width, i, tpr, g);
 #pragma unroll
-  for (int k = 0; k < NC * 8; ++k) v[k] = v[k] * rstd * (gamma ? g[k] : 1.0f);
+  for (int k = 0; k < N; ++k) v[k] = v[k] * rstd * (gamma ? g[k] : 1.0f);
   if (beta) {
-    load_row<NC, VEC>(beta, 0, KB_DT_F32, width, i, tpr, g);
+    load_row(beta, 0, KB_DT_F32, width, i, tpr, g);
 #pragma unroll
-    for (int k = 0; k < NC * 8; ++k) v[k] += g[k];
+    for (int k = 0; k < N; ++k) v[k] += g[k];
   }
 }
 
-template <int NC, bool VEC, bool BLOCK>
+template <int N, bool BLOCK>
 __global__ void __launch_bounds__(BLOCK ? 1024 : 256) norm_residual_kernel(const NormArgs a) {
   __shared__ float red[32];
   const kb_norm_residual_desc& d = a.d;
@@ -167,60 +456,50 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 256) norm_residual_kernel(const
   const int64_t row = BLOCK ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
   if (row >= d.rows) return;  // whole warps, or the whole block
   const int w = d.width;
-  float r[NC * 8];
-  load_row<NC, VEC>(a.x, row * d.x_stride, d.stream_dtype, w, i, tpr, r);
+  float r[N];
+  load_row(a.x, row * d.x_stride, d.stream_dtype, w, i, tpr, r);
   const int64_t cond = row / d.rows_per_cond * d.cond_stride;
   if (a.y) {
-    float n[NC * 8];
-    load_row<NC, VEC>(a.y, row * d.y_stride, d.branch_dtype, w, i, tpr, n);
-    norm_row<NC, VEC, BLOCK>(n, d.post_norm, a.post_gamma, a.post_beta, d.eps, w, i, tpr, red);
+    float n[N];
+    load_row(a.y, row * d.y_stride, d.branch_dtype, w, i, tpr, n);
+    norm_row<N, BLOCK>(n, d.post_norm, a.post_gamma, a.post_beta, d.eps, w, i, tpr, red);
     if (a.gate) {
-      float g[NC * 8];
-      load_row<NC, VEC>(a.gate, cond, d.branch_dtype, w, i, tpr, g);
+      float g[N];
+      load_row(a.gate, cond, d.branch_dtype, w, i, tpr, g);
 #pragma unroll
-      for (int k = 0; k < NC * 8; ++k) {
-        float f = g[k];
-        if (d.gate_act == KB_GATE_SIGMOID) f = 1.0f / (1.0f + expf(-f));
-        else if (d.gate_act == KB_GATE_TANH) f = tanhf(f);
-        n[k] *= f;
-      }
+      for (int k = 0; k < N; ++k) n[k] *= gate_value(g[k], d.gate_act);
     }
 #pragma unroll
-    for (int k = 0; k < NC * 8; ++k) r[k] = d.res_scale * r[k] + d.branch_scale * n[k];
+    for (int k = 0; k < N; ++k) r[k] = d.res_scale * r[k] + d.branch_scale * n[k];
   } else {
 #pragma unroll
-    for (int k = 0; k < NC * 8; ++k) r[k] *= d.res_scale;
+    for (int k = 0; k < N; ++k) r[k] *= d.res_scale;
   }
-  if (a.x_out) store_row<NC, VEC>(a.x_out, row * d.x_out_stride, d.stream_dtype, w, i, tpr, r);
+  if (a.x_out) store_row(a.x_out, row * d.x_out_stride, d.stream_dtype, w, i, tpr, r);
   if (a.h) {
-    norm_row<NC, VEC, BLOCK>(r, d.pre_norm, a.pre_gamma, a.pre_beta, d.eps, w, i, tpr, red);
-    float m[NC * 8];
+    norm_row<N, BLOCK>(r, d.pre_norm, a.pre_gamma, a.pre_beta, d.eps, w, i, tpr, red);
+    float m[N];
     if (a.mod_scale) {
-      load_row<NC, VEC>(a.mod_scale, cond, d.branch_dtype, w, i, tpr, m);
+      load_row(a.mod_scale, cond, d.branch_dtype, w, i, tpr, m);
 #pragma unroll
-      for (int k = 0; k < NC * 8; ++k) r[k] *= 1.0f + m[k];
+      for (int k = 0; k < N; ++k) r[k] *= 1.0f + m[k];
     }
     if (a.mod_shift) {
-      load_row<NC, VEC>(a.mod_shift, cond, d.branch_dtype, w, i, tpr, m);
+      load_row(a.mod_shift, cond, d.branch_dtype, w, i, tpr, m);
 #pragma unroll
-      for (int k = 0; k < NC * 8; ++k) r[k] += m[k];
+      for (int k = 0; k < N; ++k) r[k] += m[k];
     }
-    store_row<NC, VEC>(a.h, row * d.h_stride, d.branch_dtype, w, i, tpr, r);
+    store_row(a.h, row * d.h_stride, d.branch_dtype, w, i, tpr, r);
   }
 }
 
-template <bool VEC>
-int launch(const NormArgs& a, cudaStream_t s) {
-  const int chunks = (a.d.width + 7) / 8, rows = a.d.rows;
-  // Rows of up to 1,024 columns take a warp each, wider ones a block with at
-  // most 16 columns per thread.
-  const int warps = rows < 8 * 148 ? 1 : 4;
-  const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(rows) + warps - 1) / warps);
-  if (chunks <= 32) norm_residual_kernel<1, VEC, false><<<grid, 32 * warps, 0, s>>>(a);
-  else if (chunks <= 64) norm_residual_kernel<2, VEC, false><<<grid, 32 * warps, 0, s>>>(a);
-  else if (chunks <= 96) norm_residual_kernel<3, VEC, false><<<grid, 32 * warps, 0, s>>>(a);
-  else if (chunks <= 128) norm_residual_kernel<4, VEC, false><<<grid, 32 * warps, 0, s>>>(a);
-  else norm_residual_kernel<2, VEC, true><<<rows, ((chunks + 1) / 2 + 31) / 32 * 32, 0, s>>>(a);
+int launch_any(const NormArgs& a, cudaStream_t s) {
+  const int rows = a.d.rows, w = a.d.width;
+  const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(rows) + 3) / 4);
+  if (w <= 256) norm_residual_kernel<8, false><<<grid, 128, 0, s>>>(a);
+  else if (w <= 512) norm_residual_kernel<16, false><<<grid, 128, 0, s>>>(a);
+  else if (w <= 1024) norm_residual_kernel<32, false><<<grid, 128, 0, s>>>(a);
+  else norm_residual_kernel<16, true><<<rows, ((w + 15) / 16 + 31) / 32 * 32, 0, s>>>(a);
   return check_cuda(cudaGetLastError(), "norm launch");
 }
 
@@ -263,8 +542,8 @@ extern "C" int kb_norm_residual(const kb_norm_residual_desc* desc, const void* x
   if (x_out && x_out == y) return bad("x_out must not be y");
   NormArgs a{d, x, y, post_gamma, post_beta, pre_gamma, pre_beta, gate, mod_scale, mod_shift, x_out, h};
   if (a.d.rows_per_cond < 1) a.d.rows_per_cond = 1;
-  // Eight columns per access need whole groups and 16-byte rows; anything
-  // else takes the kernel of single elements.
+  // Eight columns per access need whole groups and 16-byte rows, and the type
+  // pairs that streams have; anything else takes the kernel of single elements.
   bool vec = d.width % 8 == 0;
   for (const void* p : {x, y, static_cast<const void*>(post_gamma), static_cast<const void*>(post_beta),
                         static_cast<const void*>(pre_gamma), static_cast<const void*>(pre_beta), gate, mod_scale,
@@ -273,5 +552,13 @@ extern "C" int kb_norm_residual(const kb_norm_residual_desc* desc, const void* x
   vec = vec && d.x_stride % 8 == 0 && (!y || d.y_stride % 8 == 0) && (!x_out || d.x_out_stride % 8 == 0) &&
         (!h || d.h_stride % 8 == 0) && (!cond || d.cond_stride % 8 == 0);
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return vec ? launch<true>(a, s) : launch<false>(a, s);
+  if (vec && d.width <= kTypedWidth) {
+    const int x_t = d.stream_dtype, y_t = d.branch_dtype;
+    if (x_t == KB_DT_BF16 && y_t == KB_DT_BF16) return launch_typed<KB_DT_BF16, KB_DT_BF16>(a, s);
+    if (x_t == KB_DT_F16 && y_t == KB_DT_F16) return launch_typed<KB_DT_F16, KB_DT_F16>(a, s);
+    if (x_t == KB_DT_F32 && y_t == KB_DT_BF16) return launch_typed<KB_DT_F32, KB_DT_BF16>(a, s);
+    if (x_t == KB_DT_F32 && y_t == KB_DT_F16) return launch_typed<KB_DT_F32, KB_DT_F16>(a, s);
+    if (x_t == KB_DT_F32 && y_t == KB_DT_F32) return launch_typed<KB_DT_F32, KB_DT_F32>(a, s);
+  }
+  return launch_any(a, s);
 }
