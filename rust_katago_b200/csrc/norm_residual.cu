@@ -6,7 +6,7 @@
 // A group of threads (one warp, or one block for wide rows) walks a run of
 // neighbouring rows and holds a row in registers as fp32 from the first load to
 // the last store; the next row's x and y are loaded while this one is at work.
-// What rows share is folded into at most four vectors in registers, built
+// What rows share is folded into at most four vectors in shared memory, built
 // again only when the row of gate and modulation changes:
 //   r = res_scale x + G n' + C   G = branch_scale gate gamma, C = branch_scale gate beta
 //   h = A r' + B                 A = gamma' (1 + mod_scale),  B = beta' (1 + mod_scale) + mod_shift
@@ -36,6 +36,7 @@ struct NormArgs {
 // Runs of rows per resident group: a few, so that groups that finish early
 // leave little idle.
 constexpr int kRunsPerSlot = 2;
+constexpr int kResident1 = 20, kResident2 = 20;
 // ------------------------------------------------------------------ whole groups of eight columns
 // Eight columns of type DT as fp32 pairs, and back.
 template <int DT>
@@ -141,8 +142,7 @@ __device__ __forceinline__ float gate_value(float v, int act) {
 }
 
 // XT, YT: types of stream and branch.  SHIFT: 0 no shifts, 1 only B, 2 also C.
-// THREADS: 32 (a warp per row, the vectors in registers) or the most that a
-// block has (the vectors in shared memory, each thread's own columns).
+// THREADS: 32 (a warp per row) or the most that a block has.
 template <int XT, int YT, int NC, int THREADS, int SHIFT>
 __global__ void __launch_bounds__(THREADS, THREADS == 320 ? 2 : 1) norm_rows_kernel(const NormArgs a,
                                                                                    int rows_per_group) {
@@ -166,28 +166,18 @@ __global__ void __launch_bounds__(THREADS, THREADS == 320 ? 2 : 1) norm_rows_ker
   const float inv_width = 1.0f / static_cast<float>(d.width);
   int turn = 0;
 
-  // The vectors G, A, B, C: chunk c of this thread.
-  constexpr int kHeld = BLOCK ? 1 : NC;
-  float2 held[4][kHeld][4];
+  // The vectors G, A, B, C in shared memory, each thread's own columns (nothing
+  // to synchronise).  In registers they cost half the warps: 118 us instead of
+  // 99 for 92,416 x 768.
   auto keep = [&](int which, int c, const float2 (&v)[4]) {
-    if constexpr (BLOCK) {
-      float4* at = shared_vectors + (which * NC + c) * 2 * tpr + i;
-      at[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
-      at[tpr] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) held[which][c][k] = v[k];
-    }
+    float4* at = shared_vectors + (which * NC + c) * 2 * tpr + i;
+    at[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+    at[tpr] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
   };
   auto vector = [&](int which, int c, float2 (&v)[4]) {
-    if constexpr (BLOCK) {
-      const float4* at = shared_vectors + (which * NC + c) * 2 * tpr + i;
-      const float4 p = at[0], q = at[tpr];
-      v[0] = make_float2(p.x, p.y), v[1] = make_float2(p.z, p.w), v[2] = make_float2(q.x, q.y), v[3] = make_float2(q.z, q.w);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = held[which][c][k];
-    }
+    const float4* at = shared_vectors + (which * NC + c) * 2 * tpr + i;
+    const float4 p = at[0], q = at[tpr];
+    v[0] = make_float2(p.x, p.y), v[1] = make_float2(p.z, p.w), v[2] = make_float2(q.x, q.y), v[3] = make_float2(q.z, q.w);
   };
   auto vectors = [&](int64_t cond) {
 #pragma unroll
@@ -317,8 +307,8 @@ __global__ void __launch_bounds__(THREADS, THREADS == 320 ? 2 : 1) norm_rows_ker
   }
 }
 
-// Rows of up to 1,024 columns take a warp each (and a block of its own: at 150
-// to 200 registers a thread more warps fit so), wider ones a block of threads
+// Rows of up to 1,024 columns take a warp each (and a block of its own, which
+// packs best at 90 to 190 registers a thread), wider ones a block of threads
 // with 16 columns each; enough groups to fill the SMs, each with a run of
 // neighbouring rows.
 template <int XT, int YT, int NC, int THREADS, int SHIFT>
@@ -326,11 +316,13 @@ int launch_shift(const NormArgs& a, cudaStream_t s) {
   auto kern = norm_rows_kernel<XT, YT, NC, THREADS, SHIFT>;
   int dev = 0;
   cudaGetDevice(&dev);
-  int threads = 32, bytes = 0, resident = 12;
+  int threads = 32, resident = NC == 1 ? kResident1 : NC == 2 ? kResident2 : 16;
   if (THREADS > 32) {
     threads = (a.d.width / 8 + NC * 32 - 1) / (NC * 32) * 32;
-    bytes = (2 + SHIFT) * NC * threads * 32;
     resident = THREADS == 320 ? 2 : 1;
+  }
+  const int bytes = (2 + SHIFT) * NC * threads * 32;
+  if (THREADS > 32) {
     if (bytes > 48 * 1024) {
       static std::atomic<uint64_t> configured{0};
       const uint64_t bit = 1ull << (dev & 63);

@@ -6,11 +6,13 @@
 // The operator only has to read and write each element once, so HBM bounds it.
 // Each thread owns one group of VE pairs of one head for many tokens: its
 // frequencies stay in registers and nothing is shared between threads.
-// Computing sine and cosine anew for every head costs less than a table would:
-// the fp64 pipe (64 per clock and SM) does the sum over the axes and the
-// reduction to one turn exactly where fp32 would lose the low bits of long
-// positions (30,000 x a frequency of 1 already costs 1e-3 of a turn), about 5
-// operations per pair.
+// Computing sine and cosine anew for every head costs less than a table would.
+// Angles are fixed-point fractions of a turn, where whole turns drop out of
+// integer arithmetic by themselves: a frequency is 64 bits of a turn, split into
+// a high and a signed low word, and pos * high + mulhi(pos, low) is the angle to
+// 2^-32 of a turn, exact for long positions where fp32 is not (position 30,000
+// times a frequency of 1 costs fp32 1e-3).  (In fp64 the conversions bounded
+// the kernel: 92,416 tokens of 36 x 64 bf16 took 195 us.)
 #include <stdint.h>
 
 #include "kb_internal.h"
@@ -26,29 +28,46 @@ struct RopeArgs {
   const int64_t* slots;
   void* out;
   int64_t x_token, x_head, out_token, out_head, out_rows;
-  int tokens, head_dim, pairs, rotary_heads, items, per_head, freq_head_stride, f16, tokens_per_thread;
+  int tokens, head_dim, pairs, rotary_heads, items, per_head, freq_head_stride, f16;
+  int block_items, block_tokens, tokens_per_thread;
 };
+
+constexpr int kBlock = 256;  // most threads of a block
+constexpr int kBlocksPerSm = 6, kMostTokens = 32;
 
 constexpr double kInvTwoPi = 0.15915494309189533576888;
 constexpr float kTwoPi = 6.28318530717958647692f;
 
-// cos and sin of `turns` full turns, |turns| <= 1/2.  16-bit results: the
-// special-function unit on a reduced angle (absolute error about 2^-21, far
-// below their rounding); fp32 results: CUDA's sincospif.
+// A frequency in 2^-64 of a turn per position: high word, signed low word.
+struct Turns {
+  int32_t high, low;
+};
+
+__device__ __forceinline__ Turns turns_of(float freq) {
+  const double f = static_cast<double>(freq) * kInvTwoPi;
+  const double part = f - rint(f);  // whole turns per position do not show
+  const int64_t q = __double2ll_rn(part * 18446744073709551616.0);  // (+-1/2 saturates by one unit)
+  const int32_t low = static_cast<int32_t>(q);
+  return Turns{static_cast<int32_t>(static_cast<uint32_t>(q >> 32) + (low < 0)), low};
+}
+
+// cos and sin of angle * 2^-32 turns.  16-bit results: the special-function
+// unit (absolute error about 2^-21 on [-pi, pi], far below their rounding);
+// fp32 results: CUDA's sincospif.
 template <bool WIDE>
-__device__ __forceinline__ void cos_sin_turns(float turns, float& c, float& s) {
+__device__ __forceinline__ void cos_sin(int32_t angle, float& c, float& s) {
   if constexpr (WIDE) {
-    sincospif(2.0f * turns, &s, &c);
+    sincospif(static_cast<float>(angle) * 0x1p-31f, &s, &c);
   } else {
-    __sincosf(turns * kTwoPi, &s, &c);
+    __sincosf(static_cast<float>(angle) * (kTwoPi * 0x1p-32f), &s, &c);
   }
 }
 
-// VE elements at p as floats.  ALIGNED: one 8- (16-bit) or 16-byte (fp32) load.
+// VE elements in one access: 16 bytes, or a single element.
 template <typename T, int VE>
 struct Raw;
 template <>
-struct Raw<uint16_t, 4> { using type = uint2; };
+struct Raw<uint16_t, 8> { using type = uint4; };
 template <>
 struct Raw<float, 4> { using type = uint4; };
 template <>
@@ -78,15 +97,22 @@ __device__ __forceinline__ typename Raw<T, VE>::type pack(const float (&v)[VE], 
   return raw;
 }
 
+template <typename R>
+__device__ __forceinline__ R load(const R* p) {  // streamed: in place, nothing else reads it
+  return __ldcs(p);
+}
+
 // A thread's item: 2 VE elements of one head, VE of them at o0 and VE at o1.
 // KB_ROPE_HALVES: u at o0 and v at o1 for pairs o0..; KB_ROPE_PAIRS: the pairs
 // o0/2.. lie interleaved across both.  VE = 1 takes any alignment.
 template <typename T, int VE, bool HALVES, int AXES>
-__global__ void __launch_bounds__(512) rope_axes_kernel(const RopeArgs a) {
-  constexpr int kUnroll = 4;
+__global__ void __launch_bounds__(kBlock) rope_axes_kernel(const RopeArgs a) {
+  constexpr int kUnroll = 2;
   using R = typename Raw<T, VE>::type;
-  const int item = blockIdx.x * blockDim.x + threadIdx.x;
-  if (item >= a.items) return;
+  // The block's threads: its items of one token, then of the next.
+  const int sub = threadIdx.x / a.block_items;
+  const int item = blockIdx.x * a.block_items + threadIdx.x - sub * a.block_items;
+  if (sub >= a.block_tokens || item >= a.items) return;
   const int head = item / a.per_head, c = item - head * a.per_head;
   const bool f16 = a.f16;
   int o0 = 2 * VE * c, o1 = o0 + VE, rotated = 0;  // rotated: pairs of this item that turn
@@ -101,30 +127,32 @@ __global__ void __launch_bounds__(512) rope_axes_kernel(const RopeArgs a) {
       rotated = max(0, min(VE, a.pairs - c * VE));
     }
   }
-  double freq[VE][AXES];
+  Turns freq[VE][AXES];
   if (rotated) {
     const float* f = a.freqs + static_cast<int64_t>(head) * a.freq_head_stride + c * VE * AXES;
 #pragma unroll
     for (int p = 0; p < VE; ++p)
 #pragma unroll
-      for (int x = 0; x < AXES; ++x) freq[p][x] = p < rotated ? static_cast<double>(f[p * AXES + x]) * kInvTwoPi : 0.0;
+      for (int x = 0; x < AXES; ++x) freq[p][x] = p < rotated ? turns_of(f[p * AXES + x]) : Turns{0, 0};
   }
   const T* src = static_cast<const T*>(a.x) + head * a.x_head;
   T* dst = static_cast<T*>(a.out) + head * a.out_head;
-  const int step = blockDim.y;
-  int t0 = static_cast<int>(blockIdx.y) * step * a.tokens_per_thread + threadIdx.y;
-  const int end = min(static_cast<int64_t>(a.tokens), static_cast<int64_t>(t0) + static_cast<int64_t>(step) * a.tokens_per_thread);
-  for (; t0 < end; t0 += kUnroll * step) {
-    R lo[kUnroll], hi[kUnroll];
-    int pos[kUnroll][AXES];
-    int64_t row[kUnroll];
+  const int step = a.block_tokens;
+  const int64_t run = static_cast<int64_t>(step) * a.tokens_per_thread;
+  int64_t t0 = blockIdx.y * run + sub;
+  const int64_t end = min(static_cast<int64_t>(a.tokens), blockIdx.y * run + run);
+  // kUnroll tokens at a time, the next ones loaded before these are at work.
+  R lo[kUnroll], hi[kUnroll];
+  int pos[kUnroll][AXES];
+  int64_t row[kUnroll];
+  auto fetch = [&](int64_t from) {
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      const int t = t0 + u * step;
+      const int64_t t = from + u * step;
       row[u] = -1;
       if (t < end) {
-        lo[u] = *reinterpret_cast<const R*>(src + t * a.x_token + o0);
-        hi[u] = *reinterpret_cast<const R*>(src + t * a.x_token + o1);
+        lo[u] = load(reinterpret_cast<const R*>(src + t * a.x_token + o0));
+        hi[u] = load(reinterpret_cast<const R*>(src + t * a.x_token + o1));
 #pragma unroll
         for (int x = 0; x < AXES; ++x) pos[u][x] = rotated ? a.positions[static_cast<int64_t>(x) * a.tokens + t] : 0;
         row[u] = t;
@@ -134,21 +162,36 @@ __global__ void __launch_bounds__(512) rope_axes_kernel(const RopeArgs a) {
         }
       }
     }
+  };
+  fetch(t0);
+  for (; t0 < end; t0 += kUnroll * step) {
+    R now_lo[kUnroll], now_hi[kUnroll];
+    int now_pos[kUnroll][AXES];
+    int64_t now_row[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      if (row[u] < 0) continue;
-      R w0 = lo[u], w1 = hi[u];
+      now_lo[u] = lo[u], now_hi[u] = hi[u], now_row[u] = row[u];
+#pragma unroll
+      for (int x = 0; x < AXES; ++x) now_pos[u][x] = pos[u][x];
+    }
+    fetch(t0 + kUnroll * step);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      if (now_row[u] < 0) continue;
+      R w0 = now_lo[u], w1 = now_hi[u];
       if (rotated) {
         float v0[VE], v1[VE];
-        unpack<T, VE>(lo[u], f16, v0);
-        unpack<T, VE>(hi[u], f16, v1);
+        unpack<T, VE>(now_lo[u], f16, v0);
+        unpack<T, VE>(now_hi[u], f16, v1);
 #pragma unroll
         for (int p = 0; p < VE; ++p) {
-          double turns = 0.0;
+          uint32_t angle = 0;
 #pragma unroll
-          for (int x = 0; x < AXES; ++x) turns = fma(static_cast<double>(pos[u][x]), freq[p][x], turns);
+          for (int x = 0; x < AXES; ++x)
+            angle += static_cast<uint32_t>(now_pos[u][x]) * static_cast<uint32_t>(freq[p][x].high) +
+                     static_cast<uint32_t>(__mulhi(now_pos[u][x], freq[p][x].low));
           float cs, sn;
-          cos_sin_turns<sizeof(T) == 4>(static_cast<float>(turns - rint(turns)), cs, sn);
+          cos_sin<sizeof(T) == 4>(static_cast<int32_t>(angle), cs, sn);
           // element indices of the pair (u, v) in the concatenation [v0 | v1]
           float* pu = HALVES || 2 * p < VE ? &v0[HALVES ? p : (2 * p) % VE] : &v1[(2 * p) % VE];
           float* pv = HALVES ? &v1[p] : 2 * p + 1 < VE ? &v0[(2 * p + 1) % VE] : &v1[(2 * p + 1) % VE];
@@ -160,8 +203,8 @@ __global__ void __launch_bounds__(512) rope_axes_kernel(const RopeArgs a) {
         w0 = pack<T, VE>(v0, f16);
         w1 = pack<T, VE>(v1, f16);
       }
-      *reinterpret_cast<R*>(dst + row[u] * a.out_token + o0) = w0;
-      *reinterpret_cast<R*>(dst + row[u] * a.out_token + o1) = w1;
+      *reinterpret_cast<R*>(dst + now_row[u] * a.out_token + o0) = w0;
+      *reinterpret_cast<R*>(dst + now_row[u] * a.out_token + o1) = w1;
     }
   }
 }
@@ -172,21 +215,22 @@ int launch(RopeArgs a, int heads, int axes, cudaStream_t stream) {
   a.items = heads * a.per_head;
   int dev = 0;
   cudaGetDevice(&dev);
-  const int nbx = (a.items + 511) / 512;
-  const int bx = ((a.items + nbx - 1) / nbx + 31) / 32 * 32;
-  const int by = bx >= 256 ? 1 : 256 / bx;
+  const int nbx = (a.items + kBlock - 1) / kBlock;
+  a.block_items = (a.items + nbx - 1) / nbx;
+  a.block_tokens = kBlock / a.block_items;
+  if (a.block_tokens > a.tokens) a.block_tokens = a.tokens;
   // Tokens per thread: enough to reuse its frequencies, few enough that every
   // SM gets several blocks.
-  const int64_t groups = (static_cast<int64_t>(a.tokens) + by - 1) / by;
-  int64_t tpt = groups * nbx / (16 * num_sms(dev));
-  tpt = tpt < 1 ? 1 : tpt > 16 ? 16 : tpt;
+  const int64_t groups = (static_cast<int64_t>(a.tokens) + a.block_tokens - 1) / a.block_tokens;
+  int64_t tpt = groups * nbx / (kBlocksPerSm * num_sms(dev));
+  tpt = tpt < 1 ? 1 : tpt > kMostTokens ? kMostTokens : tpt;
   int64_t gy = (groups + tpt - 1) / tpt;
   if (gy > 65535) {
     tpt = (groups + 65534) / 65535;
     gy = (groups + tpt - 1) / tpt;
   }
   a.tokens_per_thread = static_cast<int>(tpt);
-  const dim3 grid(nbx, static_cast<unsigned>(gy)), block(bx, by);
+  const dim3 grid(nbx, static_cast<unsigned>(gy)), block((a.block_items * a.block_tokens + 31) / 32 * 32);
   switch (axes) {
     case 1: rope_axes_kernel<T, VE, HALVES, 1><<<grid, block, 0, stream>>>(a); break;
     case 2: rope_axes_kernel<T, VE, HALVES, 2><<<grid, block, 0, stream>>>(a); break;
@@ -241,15 +285,15 @@ extern "C" int kb_rope_axes(const void* x, int dtype, int tokens, int heads, int
   a.freq_head_stride = freq_heads == 1 ? 0 : pairs * axes;
   a.f16 = dtype == KB_DT_F16;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  // Four elements per access need 8- or 16-byte addresses and whole groups;
+  // 16 bytes per access need such addresses and whole groups of 2 VE elements;
   // anything else takes the kernel of single elements.
-  const uintptr_t align = 4 * es;
-  const bool vec = head_dim % 8 == 0 && x_token % 4 == 0 && x_head % 4 == 0 && out_token % 4 == 0 &&
-                   out_head % 4 == 0 && reinterpret_cast<uintptr_t>(x) % align == 0 &&
-                   reinterpret_cast<uintptr_t>(out) % align == 0 && (layout == KB_ROPE_PAIRS || pairs % 4 == 0);
+  const int ve = 16 / es;
+  const bool vec = head_dim % (2 * ve) == 0 && x_token % ve == 0 && x_head % ve == 0 && out_token % ve == 0 &&
+                   out_head % ve == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(out) % 16 == 0 && (layout == KB_ROPE_PAIRS || pairs % ve == 0);
   const bool halves = layout == KB_ROPE_HALVES;
   if (es == 2) {
-    if (vec) return halves ? launch<uint16_t, 4, true>(a, heads, axes, s) : launch<uint16_t, 4, false>(a, heads, axes, s);
+    if (vec) return halves ? launch<uint16_t, 8, true>(a, heads, axes, s) : launch<uint16_t, 8, false>(a, heads, axes, s);
     return halves ? launch<uint16_t, 1, true>(a, heads, axes, s) : launch<uint16_t, 1, false>(a, heads, axes, s);
   }
   if (vec) return halves ? launch<float, 4, true>(a, heads, axes, s) : launch<float, 4, false>(a, heads, axes, s);
