@@ -23,25 +23,40 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
+import struct
 
 import numpy as np
 import torch
 
 from . import _capi
 from ._capi import call
-from .int8 import _ptr, _stream
 
 _DTYPES = {torch.float32: _capi.DT_F32, torch.float16: _capi.DT_F16, torch.bfloat16: _capi.DT_BF16}
 _LAYOUTS = {"pairs": _capi.ROPE_PAIRS, "halves": _capi.ROPE_HALVES}
 _NORMS = {None: _capi.NORM_NONE, "rms": _capi.NORM_RMS, "layer": _capi.NORM_LAYER}
 _GATES = {"linear": _capi.GATE_LINEAR, "sigmoid": _capi.GATE_SIGMOID, "tanh": _capi.GATE_TANH}
 
+# kb_norm_residual_desc and kb_diff_attention_desc as bytes: packing them takes a
+# third of the time of filling a ctypes structure, and a call on one token is
+# mostly this file's time.
+_NORM_DESC = struct.Struct("@8i3f5q")
+_DIFF_DESC = struct.Struct("@9i3f15q")
+assert _NORM_DESC.size == ctypes.sizeof(_capi.NormResidualDesc)
+assert _DIFF_DESC.size == ctypes.sizeof(_capi.DiffAttentionDesc)
 
-def _on(stream, device):
-    """The context in which tensors are allocated for a call on `stream`."""
+
+# What torch.cuda.current_device() and current_stream().cuda_stream return, without
+# the 10 us of their wrappers.
+_current_device = torch._C._cuda_getDevice
+_current_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _raw(stream, device):
+    """The cudaStream_t of `stream` (None: the current stream) as an integer."""
     if stream is None:
-        return contextlib.nullcontext()
-    return torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream)
+        return _current_stream(device)
+    return stream if isinstance(stream, int) else stream.cuda_stream
 
 
 def _lookup(table, key, what):
@@ -51,28 +66,45 @@ def _lookup(table, key, what):
         raise ValueError(f"{what} must be one of {list(table)}, got {key!r}") from None
 
 
-def _check(t, what, shape, dtype, device, inner=True):
-    """Raise unless `t` has this shape (None: any extent), type and device and a contiguous last dimension."""
+def _device(t, what):
+    """The device index of a CUDA tensor on the current device."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{what} must be a tensor")
-    if t.dtype != dtype:
-        raise TypeError(f"{what} must be {dtype}, got {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{what} must be on {device}, got {t.device}")
-    if len(t.shape) != len(shape) or any(w is not None and w != g for w, g in zip(shape, t.shape)):
-        raise ValueError(f"{what} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-    if inner and t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError(f"{what}'s last dimension must be contiguous")
-
-
-def _cuda(t, what):
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{what} must be a tensor")
-    if t.device.type != "cuda":
+    index = t.get_device()
+    if index < 0:
         raise ValueError(f"{what} must be a CUDA tensor")
-    if t.device.index != torch.cuda.current_device():
+    if index != _current_device():
         raise ValueError(f"{what} must be on the current device")
-    return t.device
+    return index
+
+
+def _check(t, what, shape, dtype, device):
+    """The address of `t`; raises unless it has this shape, type and device and a contiguous last dimension."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{what} must be a tensor")
+    if t.dtype is not dtype:
+        raise TypeError(f"{what} must be {dtype}, got {t.dtype}")
+    if t.get_device() != device:
+        raise ValueError(f"{what} must be on device {device}, got {t.device}")
+    if t.shape != shape:
+        raise ValueError(f"{what} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise ValueError(f"{what}'s last dimension must be contiguous")
+    return t.data_ptr()
+
+
+def _on(stream, device):
+    """The context in which tensors are allocated for a call on `stream`."""
+    if stream is None:
+        return contextlib.nullcontext()
+    return torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream)
+
+
+def _empty(like, shape, dtype, stream, device):
+    if stream is None:
+        return like.new_empty(shape, dtype=dtype)
+    with _on(stream, device):
+        return like.new_empty(shape, dtype=dtype)
 
 
 def rope_axes(x, positions, freqs, out=None, *, rotary_heads=None, layout="pairs", slots=None, stream=None):
@@ -84,28 +116,34 @@ def rope_axes(x, positions, freqs, out=None, *, rotary_heads=None, layout="pairs
     With slots (int64 [tokens]) token t goes to row slots[t] of out [rows,
     heads, head_dim] (a cache), rows outside it are skipped.  Returns out.
     """
-    device = _cuda(x, "x")
-    dtype = _lookup(_DTYPES, x.dtype, "x's dtype")
-    _check(x, "x", (None, None, None), x.dtype, device)
-    tokens, heads, head_dim = x.shape
-    rotary = heads if rotary_heads is None else rotary_heads
-    _check(positions, "positions", (None, tokens), torch.int32, device)
-    axes = positions.shape[0]
-    _check(freqs, "freqs", (None, None, axes), torch.float32, device)
+    device = _device(x, "x")
+    dtype = x.dtype
+    kind = _lookup(_DTYPES, dtype, "x's dtype")
+    if x.dim() != 3 or freqs.dim() != 3:
+        raise ValueError("x must be [tokens, heads, head_dim] and freqs [heads, pairs, axes]")
+    shape = x.shape
+    tokens, heads, head_dim = shape
+    freq_heads, pairs, axes = freqs.shape
+    xp = _check(x, "x", shape, dtype, device)
+    pp = _check(positions, "positions", (axes, tokens), torch.int32, device)
+    fp = _check(freqs, "freqs", (freq_heads, pairs, axes), torch.float32, device)
     if not positions.is_contiguous() or not freqs.is_contiguous():
         raise ValueError("positions and freqs must be contiguous")
+    sp = rows = 0
     if out is None:
         if slots is not None:
             raise ValueError("slots need an out to write to")
-        with _on(stream, device):
-            out = torch.empty((tokens, heads, head_dim), dtype=x.dtype, device=device)
-    _check(out, "out", (None if slots is not None else tokens, heads, head_dim), x.dtype, device)
-    if slots is not None:
-        _check(slots, "slots", (tokens,), torch.int64, device)
+        out = _empty(x, shape, dtype, stream, device)
+        op = out.data_ptr()
+    else:
+        rows = out.shape[0]
+        op = _check(out, "out", shape if slots is None else (rows, heads, head_dim), dtype, device)
+        if slots is not None:
+            sp = _check(slots, "slots", (tokens,), torch.int64, device)
     xs, os = x.stride(), out.stride()
-    call("kb_rope_axes", x.data_ptr(), dtype, tokens, heads, head_dim, xs[0], xs[1], positions.data_ptr(), axes,
-         freqs.data_ptr(), freqs.shape[0], freqs.shape[1], rotary, _lookup(_LAYOUTS, layout, "layout"), _ptr(slots),
-         out.shape[0], out.data_ptr(), os[0], os[1], _stream(stream))
+    call("kb_rope_axes", xp, kind, tokens, heads, head_dim, xs[0], xs[1], pp, axes, fp, freq_heads, pairs,
+         heads if rotary_heads is None else rotary_heads, _lookup(_LAYOUTS, layout, "layout"), sp, rows, op, os[0],
+         os[1], _raw(stream, device))
     return out
 
 
@@ -122,54 +160,71 @@ def norm_residual(x, y=None, *, post=None, pre=None, post_gamma=None, post_beta=
     (h_dtype without y) or None, row r using row r // rows_per_cond.  x_out may
     be x and h may be y (in place); False leaves an output out.  Returns (x_out, h).
     """
-    device = _cuda(x, "x")
-    _check(x, "x", (None, None), x.dtype, device)
-    rows, width = x.shape
-    stream_dtype = _lookup(_DTYPES, x.dtype, "x's dtype")
+    device = _device(x, "x")
+    dtype = x.dtype
+    stream_kind = _lookup(_DTYPES, dtype, "x's dtype")
+    shape = x.shape
+    if len(shape) != 2:
+        raise ValueError("x must be [rows, width]")
+    rows, width = shape
+    xp = _check(x, "x", shape, dtype, device)
+    yp = y_stride = 0
     if y is not None:
         if h_dtype is not None and h_dtype != y.dtype:
             raise TypeError("h has y's type")
         h_dtype = y.dtype
-        _check(y, "y", (rows, width), h_dtype, device)
+        yp = _check(y, "y", shape, h_dtype, device)
+        y_stride = y.stride(0)
     elif h_dtype is None:
-        h_dtype = x.dtype
-    branch_dtype = _lookup(_DTYPES, h_dtype, "h's dtype")
+        h_dtype = dtype
+    branch_kind = _lookup(_DTYPES, h_dtype, "h's dtype")
     if rows_per_cond < 1:
         raise ValueError("rows_per_cond must be positive")
-    for t, what in ((post_gamma, "post_gamma"), (post_beta, "post_beta"), (pre_gamma, "pre_gamma"), (pre_beta, "pre_beta")):
-        if t is not None:
-            _check(t, what, (width,), torch.float32, device)
-    cond_stride = None
-    for t, what in ((gate, "gate"), (mod_scale, "mod_scale"), (mod_shift, "mod_shift")):
-        if t is not None:
-            _check(t, what, (-(-rows // rows_per_cond), width), h_dtype, device)
-            stride = t.stride(0) if t.shape[0] > 1 else 0
-            if cond_stride is not None and stride != cond_stride:
-                raise ValueError("gate, mod_scale and mod_shift must have equal strides")
-            cond_stride = stride
-    with _on(stream, device):
-        if x_out is None:
-            x_out = torch.empty((rows, width), dtype=x.dtype, device=device)
-        if h is None:
-            h = torch.empty((rows, width), dtype=h_dtype, device=device)
-    x_out = None if x_out is False else x_out
-    h = None if h is False else h
-    if x_out is not None:
-        _check(x_out, "x_out", (rows, width), x.dtype, device)
-    if h is not None:
-        _check(h, "h", (rows, width), h_dtype, device)
-
-    def row_stride(t):  # rows of a single-row tensor never step
-        return 0 if t is None else t.stride(0) if rows > 1 else width
-
-    desc = _capi.NormResidualDesc(
-        rows, width, stream_dtype, branch_dtype, _lookup(_NORMS, post, "post"), _lookup(_NORMS, pre, "pre"),
-        _lookup(_GATES, gate_act, "gate_act"), rows_per_cond, res_scale, branch_scale, eps, row_stride(x), row_stride(y),
-        row_stride(x_out), row_stride(h), cond_stride or 0)
-    call("kb_norm_residual", ctypes.byref(desc), x.data_ptr(), _ptr(y), _ptr(post_gamma), _ptr(post_beta),
-         _ptr(pre_gamma), _ptr(pre_beta), _ptr(gate), _ptr(mod_scale), _ptr(mod_shift), _ptr(x_out), _ptr(h),
-         _stream(stream))
+    affine = [0 if t is None else _check(t, what, (width,), torch.float32, device)
+              for t, what in ((post_gamma, "post_gamma"), (post_beta, "post_beta"), (pre_gamma, "pre_gamma"),
+                              (pre_beta, "pre_beta"))]
+    cond, cond_stride = (0, 0, 0), None
+    if gate is not None or mod_scale is not None or mod_shift is not None:
+        cond = []
+        cond_rows = -(-rows // rows_per_cond)
+        for t, what in ((gate, "gate"), (mod_scale, "mod_scale"), (mod_shift, "mod_shift")):
+            cond.append(0 if t is None else _check(t, what, (cond_rows, width), h_dtype, device))
+            if t is not None:
+                if cond_stride is not None and t.stride(0) != cond_stride and cond_rows > 1:
+                    raise ValueError("gate, mod_scale and mod_shift must have equal strides")
+                cond_stride = t.stride(0)
+    xo_p = xo_stride = h_p = h_stride = 0
+    if x_out is None:
+        x_out = _empty(x, shape, dtype, stream, device)
+        xo_p, xo_stride = x_out.data_ptr(), width
+    elif x_out is False:
+        x_out = None
+    else:
+        xo_p, xo_stride = _check(x_out, "x_out", shape, dtype, device), x_out.stride(0)
+    if h is None:
+        h = _empty(x, shape, h_dtype, stream, device)
+        h_p, h_stride = h.data_ptr(), width
+    elif h is False:
+        h = None
+    else:
+        h_p, h_stride = _check(h, "h", shape, h_dtype, device), h.stride(0)
+    x_stride = x.stride(0)
+    if rows <= 1:  # the strides of single rows are never used
+        x_stride = y_stride = xo_stride = h_stride = width
+    desc = _NORM_DESC.pack(
+        rows, width, stream_kind, branch_kind, _lookup(_NORMS, post, "post"), _lookup(_NORMS, pre, "pre"),
+        _lookup(_GATES, gate_act, "gate_act"), rows_per_cond, res_scale, branch_scale, eps, x_stride, y_stride,
+        xo_stride, h_stride, cond_stride or 0)
+    call("kb_norm_residual", desc, xp, yp, *affine, *cond, xo_p, h_p, _raw(stream, device))
     return x_out, h
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(desc, device):
+    """Scratch that a descriptor needs on a device (its number of SMs matters)."""
+    need = ctypes.c_size_t()
+    call("kb_diff_attention_workspace", desc, ctypes.byref(need))
+    return need.value
 
 
 def diff_attention(q, k, v, lam, *, gamma=None, out_scale=1.0, eps=1e-5, scale=None, causal=False, window=0,
@@ -184,42 +239,40 @@ def diff_attention(q, k, v, lam, *, gamma=None, out_scale=1.0, eps=1e-5, scale=N
     keeps the last `window` keys of each.  Queries that see no key give zeros.
     Returns out [batch, q_len, heads, 2 d].
     """
-    device = _cuda(q, "q")
-    if q.dtype not in (torch.float16, torch.bfloat16):
-        raise TypeError(f"q must be float16 or bfloat16, got {q.dtype}")
-    _check(q, "q", (None, None, None, 2, None), q.dtype, device)
+    device = _device(q, "q")
+    dtype = q.dtype
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
+        raise TypeError(f"q must be float16 or bfloat16, got {dtype}")
+    if q.dim() != 5 or k.dim() != 5:
+        raise ValueError("q and k must be [batch, tokens, heads, 2, d]")
     batch, q_len, heads, _, d = q.shape
-    _check(k, "k", (batch, None, None, 2, d), q.dtype, device)
-    kv_len, kv_heads = k.shape[1:3]
-    _check(v, "v", (batch, kv_len, kv_heads, 2 * d), q.dtype, device)
-    _check(lam, "lam", (heads,), torch.float32, device)
-    if gamma is not None:
-        _check(gamma, "gamma", (2 * d,), torch.float32, device)
-    if kv_lens is not None:
-        _check(kv_lens, "kv_lens", (batch,), torch.int32, device)
-    mask_batch = 0
+    _, kv_len, kv_heads, _, _ = k.shape
+    qp = _check(q, "q", (batch, q_len, heads, 2, d), dtype, device)
+    kp = _check(k, "k", (batch, kv_len, kv_heads, 2, d), dtype, device)
+    vp = _check(v, "v", (batch, kv_len, kv_heads, 2 * d), dtype, device)
+    lp = _check(lam, "lam", (heads,), torch.float32, device)
+    gp = 0 if gamma is None else _check(gamma, "gamma", (2 * d,), torch.float32, device)
+    np_ = 0 if kv_lens is None else _check(kv_lens, "kv_lens", (batch,), torch.int32, device)
+    mp = mask_batch = 0
     if key_mask is not None:
-        if key_mask.dtype != torch.bool:
-            _check(key_mask, "key_mask", (batch, kv_len), torch.uint8, device)
-        else:
-            _check(key_mask, "key_mask", (batch, kv_len), torch.bool, device)
+        mp = _check(key_mask, "key_mask", (batch, kv_len),
+                    torch.bool if key_mask.dtype is torch.bool else torch.uint8, device)
         mask_batch = key_mask.stride(0)
     if out is None:
-        with _on(stream, device):
-            out = torch.empty((batch, q_len, heads, 2 * d), dtype=q.dtype, device=device)
-    _check(out, "out", (batch, q_len, heads, 2 * d), q.dtype, device)
-    desc = _capi.DiffAttentionDesc(
-        _DTYPES[q.dtype], batch, q_len, kv_len, heads, kv_heads, d, bool(causal), window,
+        out = _empty(q, (batch, q_len, heads, 2 * d), dtype, stream, device)
+        op = out.data_ptr()
+    else:
+        op = _check(out, "out", (batch, q_len, heads, 2 * d), dtype, device)
+    desc = _DIFF_DESC.pack(
+        _DTYPES[dtype], batch, q_len, kv_len, heads, kv_heads, d, bool(causal), window,
         d**-0.5 if scale is None else scale, out_scale, eps, *q.stride()[:4], *k.stride()[:4], *v.stride()[:3],
         *out.stride()[:3], mask_batch)
-    ref, need = ctypes.byref(desc), ctypes.c_size_t()
-    call("kb_diff_attention_workspace", ref, ctypes.byref(need))
-    work = None
-    if need.value:
-        with _on(stream, device):
-            work = torch.empty(need.value, dtype=torch.uint8, device=device)
-    call("kb_diff_attention", ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), _ptr(gamma),
-         _ptr(kv_lens), _ptr(key_mask), out.data_ptr(), _ptr(work), need.value, _ptr(status), _stream(stream))
+    need, wp = _workspace_bytes(desc, device), 0
+    if need:
+        work = _empty(q, need, torch.uint8, stream, device)
+        wp = work.data_ptr()
+    call("kb_diff_attention", desc, qp, kp, vp, lp, gp, np_, mp, op, wp, need,
+         0 if status is None else status.data_ptr(), _raw(stream, device))
     return out
 
 

@@ -57,10 +57,13 @@ __global__ void __launch_bounds__(128) diff_combine_kernel(const DiffArgs a, int
 struct Plan {
   bool few = false;
   int splits = 1;
+  bool joined = false;  // by the kernel itself: no workspace
 };
 
 constexpr int kFewRows = 16;
 constexpr int kFewKeys = 128;  // keys per block of four warps, at least
+constexpr int kFewBlocks = 8;  // blocks per SM to aim for (two are resident)
+constexpr int kClusterKeys = 4096;
 constexpr int kTileKeys = 128;
 constexpr int kTilesPerSplit = 4;
 
@@ -74,10 +77,14 @@ Plan make_plan(const kb_diff_attention_desc& d) {
   if (d.window && keys > static_cast<int64_t>(d.window) + d.q_len) keys = static_cast<int64_t>(d.window) + d.q_len;
   if (p.few) {
     const int64_t units = static_cast<int64_t>(d.batch) * d.kv_heads;
-    const int64_t want = (3 * static_cast<int64_t>(num_sms(dev)) + units - 1) / units;
     const int64_t most = (keys + kFewKeys - 1) / kFewKeys;
-    const int64_t s = want < most ? want : most;
+    int64_t s = (kFewBlocks * static_cast<int64_t>(num_sms(dev)) + units - 1) / units;
+    // A cluster's worth serves when it gives every SM a block, or when the
+    // keys are so few that the second launch would cost more.
+    if (s > kMostCluster && (units * kMostCluster >= num_sms(dev) || keys <= kClusterKeys)) s = kMostCluster;
+    if (s > most) s = most;
     p.splits = static_cast<int>(s < 1 ? 1 : s > 1024 ? 1024 : s);
+    p.joined = p.splits <= kMostCluster;
   } else {
     const int64_t tiles = (keys + kTileKeys - 1) / kTileKeys;
     const int64_t units = static_cast<int64_t>(d.batch) * d.heads * ((d.q_len + 127) / 128);
@@ -154,7 +161,7 @@ extern "C" int kb_diff_attention_workspace(const kb_diff_attention_desc* desc, s
   *bytes = 0;
   if (desc->batch == 0 || desc->q_len == 0) return KB_OK;
   const Plan p = make_plan(*desc);
-  if (p.splits > 1) *bytes = partial_bytes(*desc, p.splits, nullptr);
+  if (p.splits > 1 && !p.joined) *bytes = partial_bytes(*desc, p.splits, nullptr);
   return KB_OK;
 }
 
@@ -181,14 +188,14 @@ extern "C" int kb_diff_attention(const kb_diff_attention_desc* desc, const uint1
   DiffArgs a = make_diff_args(d, q, k, v, lambda, gamma, kv_lens, key_mask, out);
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const Plan p = make_plan(d);
-  if (p.splits > 1) {
+  if (need) {
     size_t at = 0;
     partial_bytes(d, p.splits, &at);
     a.part_ml = static_cast<float2*>(workspace);
     a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + at);
   }
   const int rc2 = p.few ? diff_decode_launch(a, p.splits, s) : diff_tc_launch(a, p.splits, status, s);
-  return rc2 || p.splits == 1 ? rc2 : diff_combine_launch(a, p.splits, s);
+  return rc2 || !need ? rc2 : diff_combine_launch(a, p.splits, s);
 }
 
 extern "C" int kb_diff_lambda(const float* q1, const float* k1, const float* q2, const float* k2, int heads,

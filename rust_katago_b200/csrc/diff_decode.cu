@@ -20,11 +20,15 @@
 // unrounded P in fp32.  The running maximum moves only when a score exceeds it
 // by 2^8, so most steps skip the reduction over keys and the rescaling.
 //
-// Keys are split over blocks (partial results through the workspace, joined by
-// diff_combine) and within a block over its warps (joined in shared memory), in
-// a fixed order: results do not depend on timing.
+// Keys are split over blocks and within a block over its warps.  The warps'
+// parts are joined in shared memory; the blocks' parts through distributed
+// shared memory when the blocks of a tile form a cluster (up to eight: one
+// launch, no workspace), else through the workspace by diff_combine.  Every join
+// is in a fixed order: results do not depend on timing.
 #include <math.h>
 #include <stdint.h>
+
+#include <atomic>
 
 #include "kb_diff.cuh"
 #include "kb_internal.h"
@@ -69,11 +73,27 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return r;
 }
 
+// Four floats at the same shared-memory address in block `rank` of the cluster.
+__device__ __forceinline__ float4 load_peer(const float* p, uint32_t rank) {
+  uint32_t at;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+  return v;
+}
+
+// All threads of all blocks of the cluster.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
-// NR: 8-row tiles per warp.
-template <int D, int NR, bool F16>
-__global__ void __launch_bounds__(32 * kWarps, NR == 1 ? 3 : 2) diff_decode_kernel(const DiffArgs a, int splits,
+// NR: 8-row tiles per warp.  (Two blocks per SM: three left 168 registers and
+// spilled, 231 instead of 189 us for 64 tokens on 8,192 keys.)
+template <int D, int NR, bool F16, bool CLUSTER>
+__global__ void __launch_bounds__(32 * kWarps, 2) diff_decode_kernel(const DiffArgs a, int splits,
                                                                                       int row_tiles) {
   constexpr int kCh = D / 32;   // 16-byte pieces per thread of a K row, and of half a V row
   constexpr int kKs = D / 16;   // steps of the score product
@@ -303,6 +323,9 @@ __global__ void __launch_bounds__(32 * kWarps, NR == 1 ? 3 : 2) diff_decode_kern
   __syncthreads();
   // One warp per row joins the warps' parts; lanes hold kDv / 32 dims.
   constexpr int kE = kDv / 32;
+  // CLUSTER: this block's parts, {m, l} of both maps and the sums of each row.
+  float* joined = reinterpret_cast<float*>(ml + kWarps * kRows * 2);
+  float4* joined_ml = reinterpret_cast<float4*>(joined + kRows * 2 * kDv);
   for (int row = warp; row < rows; row += kWarps) {
     const int r = r0 + row, i = r / share, h = hk * share + r % share;
     float acc[2][kE], mm[2], ll[2];
@@ -323,31 +346,104 @@ __global__ void __launch_bounds__(32 * kWarps, NR == 1 ? 3 : 2) diff_decode_kern
         for (int e = 0; e < kE; ++e) acc[m][e] = fmaf(f, src[e], acc[m][e]);
       }
     }
-    if (splits == 1) {
+    if constexpr (CLUSTER) {
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int e = 0; e < kE; ++e) joined[(row * 2 + m) * kDv + lane * kE + e] = acc[m][e];
+      if (lane == 0) joined_ml[row] = make_float4(mm[0], ll[0], mm[1], ll[1]);
+    } else if (splits == 1) {
       finish_row<kE>(a, b, i, h, lane, acc, ll);
     } else {
       write_partial<kE>(a, splits, split, b, i, h, lane, acc, mm, ll);
     }
   }
+  if constexpr (CLUSTER) {
+    // A warp of some block of the cluster joins each row: 16 lanes a map, kDv / 16
+    // dims each, then the lanes of map 1 hand theirs over.
+    cluster_sync();
+    for (int row = split * kWarps + warp; row < rows; row += kWarps * splits) {
+      const int r = r0 + row, i = r / share, h = hk * share + r % share;
+      float acc[2][kE], ll[2];
+      constexpr int kPer = kDv / 16;
+      const int m = lane >> 4, at = (row * 2 + m) * kDv + (lane & 15) * kPer;
+      float top = -INFINITY, sum = 0.0f, o[kPer];
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) o[e] = 0.0f;
+      for (int s = 0; s < splits; ++s) {
+        const float4 v = load_peer(reinterpret_cast<const float*>(joined_ml + row), s);
+        top = fmaxf(top, m ? v.z : v.x);
+      }
+      for (int s = 0; s < splits; ++s) {
+        const float4 v = load_peer(reinterpret_cast<const float*>(joined_ml + row), s);
+        const float ms = m ? v.z : v.x, ls = m ? v.w : v.y;
+        const float f = ms == -INFINITY ? 0.0f : exp2_fast(ms - top);
+        sum += f * ls;
+#pragma unroll
+        for (int e = 0; e < kPer; e += 4) {
+          const float4 p = load_peer(joined + at + e, s);
+          o[e] = fmaf(f, p.x, o[e]), o[e + 1] = fmaf(f, p.y, o[e + 1]);
+          o[e + 2] = fmaf(f, p.z, o[e + 2]), o[e + 3] = fmaf(f, p.w, o[e + 3]);
+        }
+      }
+      // to kE dims of both maps per lane: dims lane kE.. are half of lane / 2's
+      ll[0] = __shfl_sync(0xffffffffu, sum, 0), ll[1] = __shfl_sync(0xffffffffu, sum, 16);
+#pragma unroll
+      for (int e = 0; e < kE; ++e) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const float lower = __shfl_sync(0xffffffffu, o[e], 16 * t + (lane >> 1));
+          const float upper = __shfl_sync(0xffffffffu, o[e + kE], 16 * t + (lane >> 1));
+          acc[t][e] = lane & 1 ? upper : lower;
+        }
+      }
+      finish_row<kE>(a, b, i, h, lane, acc, ll);
+    }
+    cluster_sync();  // nobody leaves while its shared memory is read
+  }
 }
 
-template <int D, int NR, bool F16>
+template <int D, int NR, bool F16, bool CLUSTER>
 int launch(const DiffArgs& a, int splits, cudaStream_t s) {
-  constexpr int kBytes = kWarps * 8 * NR * 2 * (2 * D * 4 + 8);
+  constexpr int kRows = 8 * NR;
+  constexpr int kBytes = kWarps * kRows * 2 * (2 * D * 4 + 8) + (CLUSTER ? kRows * (2 * 2 * D * 4 + 16) : 0);
   const int rows = a.d.q_len * (a.d.heads / a.d.kv_heads);
-  const int row_tiles = (rows + 8 * NR - 1) / (8 * NR);
-  auto kern = diff_decode_kernel<D, NR, F16>;
+  const int row_tiles = (rows + kRows - 1) / kRows;
+  auto kern = diff_decode_kernel<D, NR, F16, CLUSTER>;
   if constexpr (kBytes > 48 * 1024) {
-    const int rc = smem_opt_in(reinterpret_cast<const void*>(kern), kBytes);
-    if (rc) return rc;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    static std::atomic<uint64_t> configured{0};
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(configured.load() & bit)) {
+      const int rc = smem_opt_in(reinterpret_cast<const void*>(kern), kBytes);
+      if (rc) return rc;
+      configured.fetch_or(bit);
+    }
   }
   const int64_t grid = static_cast<int64_t>(splits) * a.d.kv_heads * row_tiles;
   if (grid > 0x7fffffff) {
     set_error("kb_diff_attention: too many queries");
     return KB_E_INVALID;
   }
-  kern<<<dim3(static_cast<unsigned>(grid), a.d.batch), 32 * kWarps, kBytes, s>>>(a, splits, row_tiles);
-  return check_cuda(cudaGetLastError(), "differential attention (few queries) launch");
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(static_cast<unsigned>(grid), a.d.batch);
+  config.blockDim = dim3(32 * kWarps);
+  config.dynamicSmemBytes = kBytes;
+  config.stream = s;
+  cudaLaunchAttribute cluster;
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = splits, cluster.val.clusterDim.y = 1, cluster.val.clusterDim.z = 1;
+  config.attrs = &cluster;
+  config.numAttrs = CLUSTER ? 1 : 0;
+  return check_cuda(cudaLaunchKernelEx(&config, kern, a, splits, row_tiles),
+                    "differential attention (few queries) launch");
+}
+
+template <int D, int NR, bool F16>
+int launch(const DiffArgs& a, int splits, cudaStream_t s) {
+  return splits > 1 && splits <= kMostCluster ? launch<D, NR, F16, true>(a, splits, s)
+                                              : launch<D, NR, F16, false>(a, splits, s);
 }
 
 }  // namespace

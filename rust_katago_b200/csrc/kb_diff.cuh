@@ -107,6 +107,10 @@ __device__ __forceinline__ void write_partial(const DiffArgs& a, int splits, int
   }
 }
 
+// Blocks of a tile of few queries that join their keys within a cluster (the
+// portable cluster size); more of them go through the workspace.
+constexpr int kMostCluster = 8;
+
 int diff_decode_launch(const DiffArgs& a, int splits, cudaStream_t s);
 int diff_tc_launch(const DiffArgs& a, int splits, unsigned* status, cudaStream_t s);
 int diff_combine_launch(const DiffArgs& a, int splits, cudaStream_t s);
