@@ -12,17 +12,21 @@
 namespace kb {
 namespace {
 
-// Joins the parts of a row whose keys were split over blocks: one warp per
-// row, the parts in order, each weighted by 2^(its maximum - the row's).
+// Joins the parts of a row whose keys were split over blocks.  A block per row:
+// the parts are dealt to its warps in order, each weighted by 2^(its maximum -
+// the row's), and the warps' sums are added in order.  (One warp per row took
+// longer over 100 parts than the keys did.)
+constexpr int kJoinWarps = 8;
+
 template <int D>
-__global__ void __launch_bounds__(128) diff_combine_kernel(const DiffArgs a, int splits) {
+__global__ void __launch_bounds__(32 * kJoinWarps) diff_combine_kernel(const DiffArgs a, int splits) {
   constexpr int kE = 2 * D / 32;
-  const int lane = threadIdx.x & 31;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (row >= static_cast<int64_t>(a.d.batch) * a.d.q_len * a.d.heads) return;
+  __shared__ float o_sh[kJoinWarps][2][2 * D], l_sh[kJoinWarps][2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = blockIdx.x;
   const int h = static_cast<int>(row % a.d.heads);
   const int64_t bi = row / a.d.heads;
-  float acc[2][kE], mm[2], ll[2];
+  float acc[2][kE], ll[2];
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
     const float2* ml = a.part_ml + row * splits * 2 + m;
@@ -30,12 +34,12 @@ __global__ void __launch_bounds__(128) diff_combine_kernel(const DiffArgs a, int
     for (int s = lane; s < splits; s += 32) top = fmaxf(top, ml[2 * s].x);
 #pragma unroll
     for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-    mm[m] = top, ll[m] = 0.0f;
+    ll[m] = 0.0f;
 #pragma unroll
     for (int e = 0; e < kE; ++e) acc[m][e] = 0.0f;
     const float* part = a.part_o + (row * splits * 2 + m) * (2 * D) + lane * kE;
 #pragma unroll 4
-    for (int s = 0; s < splits; ++s) {
+    for (int s = warp; s < splits; s += kJoinWarps) {
       const float2 v = ml[2 * s];
       // A part that saw no key: its value sums may not have been written.  (A
       // NaN sum without a maximum is a row of NaN scores and has to go on.)
@@ -48,7 +52,20 @@ __global__ void __launch_bounds__(128) diff_combine_kernel(const DiffArgs a, int
 #pragma unroll
       for (int e = 0; e < kE; ++e) acc[m][e] = fmaf(f, o[e], acc[m][e]);
     }
+#pragma unroll
+    for (int e = 0; e < kE; ++e) o_sh[warp][m][lane * kE + e] = acc[m][e];
+    if (lane == 0) l_sh[warp][m] = ll[m];
   }
+  __syncthreads();
+  if (warp != 0) return;
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int w = 1; w < kJoinWarps; ++w) {
+      ll[m] += l_sh[w][m];
+#pragma unroll
+      for (int e = 0; e < kE; ++e) acc[m][e] += o_sh[w][m][lane * kE + e];
+    }
   finish_row<kE>(a, static_cast<int>(bi / a.d.q_len), static_cast<int>(bi % a.d.q_len), h, lane, acc, ll);
 }
 
@@ -62,7 +79,6 @@ struct Plan {
 
 constexpr int kFewRows = 16;
 constexpr int kFewKeys = 128;  // keys per block of four warps, at least
-constexpr int kFewBlocks = 8;  // blocks per SM to aim for (two are resident)
 constexpr int kClusterKeys = 4096;
 constexpr int kTileKeys = 128;
 constexpr int kTilesPerSplit = 4;
@@ -78,7 +94,10 @@ Plan make_plan(const kb_diff_attention_desc& d) {
   if (p.few) {
     const int64_t units = static_cast<int64_t>(d.batch) * d.kv_heads;
     const int64_t most = (keys + kFewKeys - 1) / kFewKeys;
-    int64_t s = (kFewBlocks * static_cast<int64_t>(num_sms(dev)) + units - 1) / units;
+    // One wave of the two blocks that an SM holds; with more tiles than that
+    // has room for, about two waves of smaller blocks, which even out lengths.
+    const int64_t slots = 2 * static_cast<int64_t>(num_sms(dev));
+    int64_t s = 2 * units <= slots ? slots / units : (2 * slots + units - 1) / units;
     // A cluster's worth serves when it gives every SM a block, or when the
     // keys are so few that the second launch would cost more.
     if (s > kMostCluster && (units * kMostCluster >= num_sms(dev) || keys <= kClusterKeys)) s = kMostCluster;
@@ -139,9 +158,9 @@ int check_desc(const kb_diff_attention_desc* desc) {
 
 int diff_combine_launch(const DiffArgs& a, int splits, cudaStream_t s) {
   const int64_t rows = static_cast<int64_t>(a.d.batch) * a.d.q_len * a.d.heads;
-  const unsigned grid = static_cast<unsigned>((rows + 3) / 4);
-  if (a.d.head_dim == 64) diff_combine_kernel<64><<<grid, 128, 0, s>>>(a, splits);
-  else diff_combine_kernel<32><<<grid, 128, 0, s>>>(a, splits);
+  const unsigned grid = static_cast<unsigned>(rows);
+  if (a.d.head_dim == 64) diff_combine_kernel<64><<<grid, 32 * kJoinWarps, 0, s>>>(a, splits);
+  else diff_combine_kernel<32><<<grid, 32 * kJoinWarps, 0, s>>>(a, splits);
   return check_cuda(cudaGetLastError(), "differential attention join launch");
 }
 

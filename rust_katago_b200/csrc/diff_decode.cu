@@ -9,13 +9,14 @@
 // (16 keys x 8 rows) and O^T = V^T P^T (16 value dims x 8 rows), so a tile is 8
 // rows wide (rows: queries x heads of the group) instead of the 16 that queries
 // as the M side would pad to.  mma.sync and not tcgen05: a tcgen05 tile is 128
-// rows of which one is used, and its operands must pass through shared memory;
-// here each thread's fragments are 16-byte pieces of the K and V rows in
-// global memory, taken straight into registers.  That needs no order of dims
-// in memory: the contraction over head dims uses the same permutation for Q,
-// and value dims come out permuted, eight neighbours per thread.  The loads of
-// the next K go out while the softmax and the value product of the current 16
-// keys run, those of the next V before the next score product.
+// rows of which one is used.  Fragments are 16-byte pieces of the K and V rows:
+// the contraction over head dims uses the same permutation for Q, and value dims
+// come out permuted, eight neighbours per thread.
+// Each warp has a ring of steps of its own in shared memory, filled by
+// asynchronous 16-byte copies kStages - 1 steps ahead, about 128 KB in flight
+// per SM, with nothing to synchronise between warps.  (Loading the fragments
+// straight into registers, one step ahead, kept half of that in flight and
+// stopped at 4.3 TB/s.)
 // P is rounded to the 16-bit type for the value product; sums are taken of the
 // unrounded P in fp32.  The running maximum moves only when a score exceeds it
 // by 2^8, so most steps skip the reduction over keys and the rescaling.
@@ -38,6 +39,9 @@ namespace kb {
 namespace {
 
 constexpr int kWarps = 4;
+// Steps of 16 keys in a warp's ring: 96 KB for a block of four warps.
+template <int D>
+constexpr int stages() { return D == 64 ? 3 : 6; }
 constexpr float kLazy = 8.0f;  // log2 of how far a score may exceed the running maximum
 
 template <bool F16>
@@ -57,6 +61,17 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
+}
+
+// 16 bytes global -> shared without registers; zeros instead unless `in`.
+__device__ __forceinline__ void copy16(uint32_t dst, const uint16_t* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Wait until at most N committed groups of this thread's copies are pending.
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 __device__ __forceinline__ uint4 load16(const uint16_t* p) {
@@ -99,7 +114,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) diff_decode_kernel(const DiffA
   constexpr int kKs = D / 16;   // steps of the score product
   constexpr int kMt = D / 8;    // 16-dim tiles of the value product
   constexpr int kRows = 8 * NR, kDv = 2 * D;
-  extern __shared__ float sm[];  // [warp][row][map]: kDv sums; then {m, l}
+  extern __shared__ __align__(128) float sm[];  // [warp][row][map]: kDv sums; then {m, l}
   const kb_diff_attention_desc& d = a.d;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int share = d.heads / d.kv_heads;
@@ -158,53 +173,79 @@ __global__ void __launch_bounds__(32 * kWarps, 2) diff_decode_kernel(const DiffA
         for (int e = 0; e < 4; ++e) o[m][t][x][e] = 0.0f;
     }
 
-  uint4 kf[2][2][kCh], vv[4][kCh];
-  const uint16_t* kbase = a.k + b * d.k_batch + hk * d.k_head + c * 8;
-  const uint16_t* vbase = a.v + b * d.v_batch + hk * d.v_head + g * 8;
-  auto load_k = [&](int j) {
+  // This warp's ring.  A step: K rows of 128 bytes (D = 64: map 0's 16 keys, then
+  // map 1's; D = 32: both maps of a key side by side), then V rows of 128 bytes
+  // (D = 64: the lower 64 dims of the keys, then the upper), 16-byte pieces
+  // swizzled by the key.
+  constexpr int kStages = stages<D>(), kKBytes = 16 * 4 * D, kStep = 2 * kKBytes;
+  uint8_t* ring = reinterpret_cast<uint8_t*>(sm) + warp * kStages * kStep;
+  const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
+  constexpr int kRowPieces = D / 4;            // pieces of a key's K (both maps), and of its V
+  constexpr int kKeysPer = 32 / kRowPieces;    // keys that 32 lanes copy at once
+  const int my_key = lane / kRowPieces, piece = lane % kRowPieces;
+  const uint16_t* kbase = a.k + b * d.k_batch + hk * d.k_head + (piece / (D / 8)) * d.k_map + piece % (D / 8) * 8;
+  const uint16_t* vbase = a.v + b * d.v_batch + hk * d.v_head + piece * 8;
+  auto fill = [&](int j, int stage) {
 #pragma unroll
-    for (int y = 0; y < 2; ++y) {
-      const int key = j + g + 8 * y;
-#pragma unroll
-      for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int x = 0; x < kCh; ++x)
-          kf[m][y][x] = key < s1 ? load16(kbase + key * d.k_token + m * d.k_map + x * 32) : make_uint4(0, 0, 0, 0);
+    for (int u = 0; u < 16 / kKeysPer; ++u) {
+      const int key = my_key + u * kKeysPer;
+      const bool in = j + key < s1;
+      const int64_t row = in ? j + key : 0;
+      const uint32_t at = ring_at + stage * kStep + ((piece >> 3) * 16 + key) * 128 + (((piece & 7) ^ (key & 7)) << 4);
+      copy16(at, kbase + row * d.k_token, in);
+      copy16(at + kKBytes, vbase + row * d.v_token, in);
     }
   };
-  // V: keys 2c, 2c + 1, 2c + 8, 2c + 9, dims 8g.. (and 64 + 8g.. for D = 64).
-  auto load_v = [&](int j) {
+  int next = s0 + 16 * warp, fill_stage = 0;
 #pragma unroll
-    for (int y = 0; y < 4; ++y) {
-      const int key = j + 2 * c + (y & 1) + 8 * (y >> 1);
-#pragma unroll
-      for (int x = 0; x < kCh; ++x)
-        vv[y][x] = key < s1 ? load16(vbase + key * d.v_token + x * 64) : make_uint4(0, 0, 0, 0);
-    }
-  };
-
-  int j = s0 + 16 * warp;
-  if (j < s1) {
-    load_k(j);
-    load_v(j);
+  for (int u = 0; u < kStages - 1; ++u, next += 16 * kWarps) {
+    if (next < s1) fill(next, fill_stage);
+    copies_commit();
+    ++fill_stage;
   }
-  for (; j < s1; j += 16 * kWarps) {
+  int stage = 0;
+  for (int j = s0 + 16 * warp; j < s1; j += 16 * kWarps) {
+    copies_wait<kStages - 2>();
+    __syncwarp();  // all lanes' copies of this step have landed, and all have left the step before
+    if (next < s1) fill(next, fill_stage);
+    copies_commit();
+    next += 16 * kWarps;
+    fill_stage = fill_stage + 1 == kStages ? 0 : fill_stage + 1;
+    const uint8_t* kt = ring + stage * kStep;
+    const uint8_t* vt = kt + kKBytes;
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+    auto k_piece = [&](int m, int key, int x) -> uint4 {
+      const int row = D == 64 ? m * 16 + key : key, p = D == 64 ? x * 4 + c : m * 4 + c;
+      return *reinterpret_cast<const uint4*>(kt + row * 128 + ((p ^ (key & 7)) << 4));
+    };
     float s[2][NR][4];
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+    for (int m = 0; m < 2; ++m) {
+      uint4 kf[2][kCh];
+#pragma unroll
+      for (int x = 0; x < kCh; ++x) kf[0][x] = k_piece(m, g, x), kf[1][x] = k_piece(m, g + 8, x);
 #pragma unroll
       for (int t = 0; t < NR; ++t) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[m][t][e] = 0.0f;
 #pragma unroll
         for (int ks = 0; ks < kKs; ++ks) {
-          const uint4 &k0 = kf[m][0][ks / 2], &k1 = kf[m][1][ks / 2];
+          const uint4 &k0 = kf[0][ks / 2], &k1 = kf[1][ks / 2];
           const uint32_t af[4] = {word(k0, 2 * (ks & 1)), word(k1, 2 * (ks & 1)), word(k0, 2 * (ks & 1) + 1),
                                   word(k1, 2 * (ks & 1) + 1)};
           mma16816<F16>(s[m][t], af, qf[m][t][ks][0], qf[m][t][ks][1]);
         }
       }
-    if (j + 16 * kWarps < s1) load_k(j + 16 * kWarps);
+    }
+    // V: keys 2c, 2c + 1, 2c + 8, 2c + 9, dims 8g.. (and 64 + 8g.. for D = 64).
+    uint4 vv[4][kCh];
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const int key = 2 * c + (y & 1) + 8 * (y >> 1);
+#pragma unroll
+      for (int x = 0; x < kCh; ++x)
+        vv[y][x] = *reinterpret_cast<const uint4*>(vt + (x * 16 + key) * 128 + ((g ^ (key & 7)) << 4));
+    }
 
     // Scores to log2 units, hidden ones to -inf; values of hidden keys to zero.
     const bool inside = j >= common_lo && j + 16 <= common_hi && mask == nullptr;
@@ -292,8 +333,9 @@ __global__ void __launch_bounds__(32 * kWarps, 2) diff_decode_kernel(const DiffA
 #pragma unroll
         for (int t = 0; t < NR; ++t) mma16816<F16>(o[m][t][x], af, pf[m][t][0], pf[m][t][1]);
     }
-    if (j + 16 * kWarps < s1) load_v(j + 16 * kWarps);
   }
+  copies_wait<0>();
+  __syncthreads();  // the ring becomes the warps' parts
 
   // Sums over the keys of the warp's lanes, then the warps' parts to shared memory.
   float2* ml = reinterpret_cast<float2*>(sm + kWarps * kRows * 2 * kDv);
@@ -406,7 +448,9 @@ __global__ void __launch_bounds__(32 * kWarps, 2) diff_decode_kernel(const DiffA
 template <int D, int NR, bool F16, bool CLUSTER>
 int launch(const DiffArgs& a, int splits, cudaStream_t s) {
   constexpr int kRows = 8 * NR;
-  constexpr int kBytes = kWarps * kRows * 2 * (2 * D * 4 + 8) + (CLUSTER ? kRows * (2 * 2 * D * 4 + 16) : 0);
+  constexpr int kJoin = kWarps * kRows * 2 * (2 * D * 4 + 8) + (CLUSTER ? kRows * (2 * 2 * D * 4 + 16) : 0);
+  constexpr int kRing = kWarps * stages<D>() * 16 * 8 * D;
+  constexpr int kBytes = kJoin > kRing ? kJoin : kRing;
   const int rows = a.d.q_len * (a.d.heads / a.d.kv_heads);
   const int row_tiles = (rows + kRows - 1) / kRows;
   auto kern = diff_decode_kernel<D, NR, F16, CLUSTER>;
