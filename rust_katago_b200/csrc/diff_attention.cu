@@ -69,15 +69,20 @@ __global__ void __launch_bounds__(32 * kJoinWarps) diff_combine_kernel(const Dif
   finish_row<kE>(a, static_cast<int>(bi / a.d.q_len), static_cast<int>(bi % a.d.q_len), h, lane, acc, ll);
 }
 
-// How a call runs: rows (queries x heads of a group) up to kFewRows by the
-// kernel for few queries, with its keys split over blocks.
+// How a call runs.  The kernel for few queries takes 16 rows (queries x heads of
+// a group) a tile and reads K and V once for each; the one for many takes 128
+// queries of one head.  Over the same keys a tile of the former costs about 3/4
+// of one of the latter (32 sequences of 2,000 keys: 20 queries 64 against 42 us,
+// 8 queries of 4 grouped heads 107 against 261 us), so the sums of tiles decide.
+// A call of few tiles and short keys is all latency, where the former is quicker
+// (120 queries on 1,000 keys, 4 heads: 15 against 22 us).
 struct Plan {
   bool few = false;
   int splits = 1;
   bool joined = false;  // by the kernel itself: no workspace
 };
 
-constexpr int kFewRows = 16;
+constexpr int kShortTiles = 36, kShortKeys = 2048;
 constexpr int kFewKeys = 128;  // keys per block of four warps, at least
 constexpr int kClusterKeys = 4096;
 constexpr int kTileKeys = 128;
@@ -86,13 +91,14 @@ constexpr int kTilesPerSplit = 4;
 Plan make_plan(const kb_diff_attention_desc& d) {
   Plan p;
   const int64_t rows = static_cast<int64_t>(d.q_len) * (d.heads / d.kv_heads);
-  p.few = rows <= kFewRows || d.kv_len == 0;
   int dev = 0;
   cudaGetDevice(&dev);
   int64_t keys = d.kv_len;
   if (d.window && keys > static_cast<int64_t>(d.window) + d.q_len) keys = static_cast<int64_t>(d.window) + d.q_len;
+  const int64_t few_tiles = (rows + 15) / 16 * d.kv_heads, many_tiles = (d.q_len + 127) / 128 * static_cast<int64_t>(d.heads);
+  p.few = few_tiles * 3 <= many_tiles * 4 || (few_tiles * d.batch <= kShortTiles && keys <= kShortKeys) || keys == 0;
   if (p.few) {
-    const int64_t units = static_cast<int64_t>(d.batch) * d.kv_heads;
+    const int64_t units = static_cast<int64_t>(d.batch) * (rows <= 8 ? d.kv_heads : few_tiles);
     const int64_t most = (keys + kFewKeys - 1) / kFewKeys;
     // One wave of the two blocks that an SM holds; with more tiles than that
     // has room for, about two waves of smaller blocks, which even out lengths.
