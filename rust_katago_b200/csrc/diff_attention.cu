@@ -86,7 +86,7 @@ constexpr int kShortTiles = 36, kShortKeys = 2048;
 constexpr int kFewKeys = 128;  // keys per block of four warps, at least
 constexpr int kClusterKeys = 4096;
 constexpr int kTileKeys = 128;
-constexpr int kTilesPerSplit = 4;
+constexpr int kTilesPerPart = 4, kMostParts = 32;
 
 Plan make_plan(const kb_diff_attention_desc& d) {
   Plan p;
@@ -111,11 +111,19 @@ Plan make_plan(const kb_diff_attention_desc& d) {
     p.splits = static_cast<int>(s < 1 ? 1 : s > 1024 ? 1024 : s);
     p.joined = p.splits <= kMostCluster;
   } else {
-    const int64_t tiles = (keys + kTileKeys - 1) / kTileKeys;
-    const int64_t units = static_cast<int64_t>(d.batch) * d.heads * ((d.q_len + 127) / 128);
-    const int64_t want = num_sms(dev) / units, most = tiles / kTilesPerSplit;
-    const int64_t s = want < most ? want : most;
-    p.splits = static_cast<int>(s < 1 ? 1 : s > 64 ? 64 : s);
+    // Parts of the keys so that the items fill the SMs evenly: rounds of items
+    // times an item's time, plus the join, in microseconds as measured (a tile
+    // of 128 keys 2, an item's start and end 2.5, the join 4 and its bytes).
+    const int64_t tiles = (keys + kTileKeys - 1) / kTileKeys, sms = num_sms(dev);
+    const int64_t units = static_cast<int64_t>(d.batch) * many_tiles;
+    const double part_bytes = static_cast<double>(d.batch) * d.q_len * d.heads * 32.0 * d.head_dim;
+    double best = 0.0;
+    for (int64_t s = 1; s <= kMostParts && (s == 1 || tiles / s >= kTilesPerPart); ++s) {
+      const double rounds = static_cast<double>((units * s + sms - 1) / sms);
+      const double us = rounds * (2.0 * static_cast<double>((tiles + s - 1) / s) + 2.5) +
+                        (s > 1 ? 4.0 + part_bytes * static_cast<double>(s) / 5e6 : 0.0);
+      if (s == 1 || us < 0.95 * best) best = us, p.splits = static_cast<int>(s);
+    }
   }
   return p;
 }

@@ -14,11 +14,12 @@
 //   warps 8-11       epilogue: the weighted difference, its norm, the output
 //   warp 12          MMA issue
 //   warp 13          TMA loads of Q, K and V
-//   warp 14          key mask bits; clears the V rows of hidden keys
+//   warp 14          limits of the keys' scores; clears the V rows of hidden keys
 //   shared memory    Q of two items, a ring of K tiles (both maps) and one of
 //                    V tiles (shared by the maps), swizzled as the MMAs read them
 //   tensor memory    S of each map (128 columns, overwritten by P as packed
-//                    16-bit pairs, the A operand of P V) and O of each map (2 D)
+//                    16-bit pairs, the A operand of P V) and O of each map (2 D),
+//                    for D = 32 of two items
 // One pass over the keys with a running maximum and sum per map.  O is rescaled
 // only when a row's maximum grows by more than 2^8 (then by the softmax
 // warps, which at that point own it: S of a tile is issued after P V of the
@@ -28,6 +29,7 @@
 // their P is 0, but 0 * NaN is not.
 // When items are too few for the SMs, the keys of an item are split over blocks
 // and diff_combine joins the parts in a fixed order.
+#include <limits.h>
 #include <math.h>
 #include <stdint.h>
 
@@ -64,14 +66,20 @@ struct Geo {
   static constexpr int kVOff = kKOff + kStages * 2 * kQk;
   static constexpr int kBarOff = kVOff + kStages * kV;
   static constexpr int kBars = 512;
-  static constexpr int kMlOff = kBarOff + kBars;    // [2 maps][128] {m, l}
-  static constexpr int kMaskOff = kMlOff + 2 * kTile * 8;  // [stage][4] words
-  static constexpr int kBytes = kMaskOff + kStages * 16 + 1024;
-  static constexpr uint32_t kO = 256, kDv = 2 * D;  // TMEM: S of map m at 128 m, O at kO + m kDv
+  // O of two items where tensor memory has room for it, so that the epilogue of
+  // one runs beside the products of the next.
+  static constexpr int kOBufs = D == 32 ? 2 : 1;
+  static constexpr int kMlOff = kBarOff + kBars;    // [O buffer][2 maps][128] {m, l}
+  static constexpr int kLimitOff = kMlOff + kOBufs * 2 * kTile * 8;  // [stage][128] limits of a key's scores
+  static constexpr int kAllOff = kLimitOff + kStages * kTile * 4;        // [stage] whether all keys are seen
+  static constexpr int kBytes = kAllOff + kStages * 4 + 1024;
+  static constexpr uint32_t kO = 256, kDv = 2 * D;  // TMEM: S of map m at 128 m, O at kO + (2 buffer + m) kDv
+  static_assert(kO + 2 * kOBufs * kDv <= kTmemCols, "tensor memory");
 };
 
 struct Items {
   int q_tiles, splits, count;
+  FastDiv by_splits, by_tiles, by_heads;  // by_tiles: causal calls by batch x heads
 };
 
 // 0 for a dimension that the strides broadcast (its tensor map extent is 1), else 1.
@@ -83,18 +91,13 @@ struct Broadcast {
 // the most keys, first; otherwise the tiles of a head together, so that its K
 // and V come from L2.
 __device__ __forceinline__ void item_of(const DiffArgs& a, const Items& it, int at, int& b, int& h, int& qt, int& split) {
-  split = at % it.splits;
-  at /= it.splits;
-  if (a.d.causal) {
-    const int bh = a.d.batch * a.d.heads;
-    qt = it.q_tiles - 1 - at / bh;
-    at %= bh;
-  } else {
-    qt = at % it.q_tiles;
-    at /= it.q_tiles;
-  }
-  h = at % a.d.heads;
-  b = at / a.d.heads;
+  uint32_t rest = it.by_splits.div(at);
+  split = at - static_cast<int>(rest) * it.splits;
+  const uint32_t outer = it.by_tiles.div(rest), inner = rest - outer * it.by_tiles.d;
+  qt = a.d.causal ? it.q_tiles - 1 - static_cast<int>(outer) : static_cast<int>(inner);
+  rest = a.d.causal ? inner : outer;
+  b = static_cast<int>(it.by_heads.div(rest));
+  h = static_cast<int>(rest) - b * a.d.heads;
 }
 
 // Key tiles [t0, t1) of an item.
@@ -104,7 +107,7 @@ __device__ __forceinline__ void tiles_of(const DiffArgs& a, const Items& it, int
   int first, last;
   key_range_n(a.d, n, qt * kTile, min(a.d.q_len, qt * kTile + kTile) - 1, first, last);
   const int lo = first / kTile, hi = last > first ? (last + kTile - 1) / kTile : lo;
-  const int per = (hi - lo + it.splits - 1) / it.splits;
+  const int per = static_cast<int>(it.by_splits.div(hi - lo + it.splits - 1));
   t0 = min(hi, lo + split * per);
   t1 = min(hi, t0 + per);
 }
@@ -221,21 +224,24 @@ __global__ void __launch_bounds__(kThreads, 1) diff_tc_kernel(const __grid_const
   uint64_t* s_full = bars + 4;        // [map] S ready                        (commit)
   uint64_t* p_full = bars + 6;        // [map][part] part of P written        (128 arrivals)
   uint64_t* pv_done = bars + 10;      // [map] P V done: P consumed           (commit)
-  uint64_t* o_full = bars + 12;       // [map] O of an item complete          (commit)
-  uint64_t* o_empty = bars + 14;      // O, maxima and sums read              (128 arrivals)
-  uint64_t* ml_full = bars + 15;      // maxima and sums of an item written   (256 arrivals)
-  uint64_t* drain = bars + 16;        // after an abort: issued MMAs done     (commit)
-  uint64_t* k_full = bars + 17;       // [stage]                              (tx bytes)
+  uint64_t* o_full = bars + 12;       // [O buffer][map] O of an item complete (commit)
+  uint64_t* o_empty = bars + 16;      // [O buffer] O, maxima and sums read   (128 arrivals)
+  uint64_t* ml_full = bars + 18;      // [O buffer] maxima and sums written   (256 arrivals)
+  uint64_t* drain = bars + 20;        // after an abort: issued MMAs done     (commit)
+  uint64_t* k_full = bars + 21;       // [stage]                              (tx bytes)
   uint64_t* k_empty = k_full + kS;    // [stage]                              (commit)
   uint64_t* v_full = k_empty + kS;    // [stage]                              (tx bytes)
   uint64_t* v_empty = v_full + kS;    // [stage]                              (commit)
   uint64_t* v_ready = v_empty + kS;   // [stage] hidden rows cleared          (32 arrivals)
-  uint64_t* bits_full = v_ready + kS; // [stage] key mask bits written        (32 arrivals)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bits_full + kS);
+  uint64_t* limit_full = v_ready + kS; // [stage] limits written             (32 arrivals)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(limit_full + kS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert((17 + 6 * kS) * 8 + 8 <= G::kBars, "barrier space");
+  static_assert((21 + 6 * kS) * 8 + 8 <= G::kBars, "barrier space");
   float2* ml = reinterpret_cast<float2*>(smem + G::kMlOff);
-  uint32_t* mask_bits = reinterpret_cast<uint32_t*>(smem + G::kMaskOff);
+  // Keys that key_mask or kv_lens hide have the limit -inf, others +inf; the
+  // smaller of score and limit hides a NaN too.
+  float* limits = reinterpret_cast<float*>(smem + G::kLimitOff);
+  int* all_seen = reinterpret_cast<int*>(smem + G::kAllOff);
 
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -246,18 +252,19 @@ __global__ void __launch_bounds__(kThreads, 1) diff_tc_kernel(const __grid_const
       mbar_init(&p_full[2 * i], kTile);
       mbar_init(&p_full[2 * i + 1], kTile);
       mbar_init(&pv_done[i], 1);
-      mbar_init(&o_full[i], 1);
+      mbar_init(&o_full[2 * i], 1);
+      mbar_init(&o_full[2 * i + 1], 1);
+      mbar_init(&o_empty[i], kTile);
+      mbar_init(&ml_full[i], 2 * kTile);
     }
     mbar_init(drain, 1);
-    mbar_init(o_empty, kTile);
-    mbar_init(ml_full, 2 * kTile);
     for (int i = 0; i < kS; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 1);
       mbar_init(&v_full[i], 1);
       mbar_init(&v_empty[i], 1);
       mbar_init(&v_ready[i], 32);
-      mbar_init(&bits_full[i], 32);
+      mbar_init(&limit_full[i], 32);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -278,7 +285,6 @@ __global__ void __launch_bounds__(kThreads, 1) diff_tc_kernel(const __grid_const
     const int map = warp >> 2, quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t o_addr = tmem + lanes + G::kO + map * G::kDv;
     const float scale = a.scale_log2;
     const uint32_t s_addr = tmem + lanes + map * 128;
     int tile = 0, busy = 0;  // tiles and items with keys so far
@@ -293,10 +299,12 @@ __global__ void __launch_bounds__(kThreads, 1) diff_tc_kernel(const __grid_const
       key_range_n(a.d, n, i, i, lo, hi);
       key_range_n(a.d, n, i1, i1, common_lo, x1);
       key_range_n(a.d, n, i0, i0, x0, common_hi);
+      const int obuf = busy % G::kOBufs;
+      const uint32_t o_addr = tmem + lanes + G::kO + (2 * obuf + map) * G::kDv;
       float m = -INFINITY, l = 0.0f;
       for (int t = t0; t < t1; ++t, ++tile) {
         const int stage = tile % kS;
-        if (!KB_WARP_WAIT(&s_full[map], tile & 1) || (has_mask && !KB_WARP_WAIT(&bits_full[stage], (tile / kS) & 1))) {
+        if (!KB_WARP_WAIT(&s_full[map], tile & 1) || (has_mask && !KB_WARP_WAIT(&limit_full[stage], (tile / kS) & 1))) {
           ok = false;
           break;
         }
@@ -306,12 +314,24 @@ __global__ void __launch_bounds__(kThreads, 1) diff_tc_kernel(const __grid_const
         for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(s + 32 * c));
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld_wait(*reinterpret_cast<uint32_t(*)[32]>(s + 32 * c));
-        if (has_mask || t * kTile < common_lo || (t + 1) * kTile > common_hi) {  // hidden keys to -inf
+        // Hidden keys to -inf: by their limits, then by the row's own bounds.
+        if (has_mask && !all_seen[stage]) {
+          const float4* limit = reinterpret_cast<const float4*>(limits + stage * kTile);
+#pragma unroll
+          for (int k = 0; k < kTile / 4; ++k) {
+            const float4 w = limit[k];
+            s[4 * k] = __float_as_uint(fminf(__uint_as_float(s[4 * k]), w.x));
+            s[4 * k + 1] = __float_as_uint(fminf(__uint_as_float(s[4 * k + 1]), w.y));
+            s[4 * k + 2] = __float_as_uint(fminf(__uint_as_float(s[4 * k + 2]), w.z));
+            s[4 * k + 3] = __float_as_uint(fminf(__uint_as_float(s[4 * k + 3]), w.w));
+          }
+        }
+        if (t * kTile < common_lo || (t + 1) * kTile > (has_mask && !a.d.causal ? INT_MAX : common_hi)) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const int base = t * kTile + 32 * c;
-            uint32_t see = bits_between(lo - base, hi - base);
-            if (has_mask) see &= mask_bits[stage * 4 + c];
+            const uint32_t see = bits_between(lo - base, hi - base);
+            if (__all_sync(0xffffffffu, see == 0xffffffffu)) continue;
 #pragma unroll
             for (int k = 0; k < 32; ++k)
               if (!(see >> k & 1u)) s[32 * c + k] = 0xff800000u;
@@ -370,103 +390,114 @@ __global__ void __launch_bounds__(kThreads, 1) diff_tc_kernel(const __grid_const
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       }
       if (!ok) break;
-      // The epilogue has read the previous item's maxima and sums.
-      if (busy > 0 && !KB_WARP_WAIT(o_empty, (busy - 1) & 1)) break;
-      ml[map * kTile + row] = make_float2(m, l);
-      mbar_arrive(ml_full);
+      // The epilogue has read the maxima and sums of the buffer's last item.
+      if (busy >= G::kOBufs && !KB_WARP_WAIT(&o_empty[obuf], (busy / G::kOBufs - 1) & 1)) break;
+      ml[(2 * obuf + map) * kTile + row] = make_float2(m, l);
+      mbar_arrive(&ml_full[obuf]);
       ++busy;
     }
   } else if (warp < kMmaWarp) {
     // ------------------------------------------------------------ epilogue
     set_regs<kRegsLaunch, kRegsEpi>();
     const int row = threadIdx.x & (kTile - 1);
-    const uint32_t o_addr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + G::kO;
     int busy = 0;
     for (int round = 0, at; (at = item_at(round)) < items.count; ++round) {
       int b, h, qt, split, n, t0, t1;
       item_of(a, items, at, b, h, qt, split);
       tiles_of(a, items, b, qt, split, n, t0, t1);
-      const int i = qt * kTile + row;
+      const int i = qt * kTile + row, obuf = busy % G::kOBufs;
+      const uint32_t o_addr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + G::kO + 2 * obuf * G::kDv;
       const bool live = i < a.d.q_len;
       const bool any = t0 < t1;
+      const float lambda = a.lambda[h];
       float2 v0 = make_float2(-INFINITY, 0.0f), v1 = v0;
       if (any) {
-        if (!KB_WARP_WAIT(ml_full, busy & 1) || !KB_WARP_WAIT(&o_full[0], busy & 1) ||
-            !KB_WARP_WAIT(&o_full[1], busy & 1))
+        const uint32_t parity = (busy / G::kOBufs) & 1;
+        if (!KB_WARP_WAIT(&ml_full[obuf], parity) || !KB_WARP_WAIT(&o_full[2 * obuf], parity) ||
+            !KB_WARP_WAIT(&o_full[2 * obuf + 1], parity))
           break;
         tc_fence_after();
-        v0 = ml[row], v1 = ml[kTile + row];
+        v0 = ml[2 * obuf * kTile + row], v1 = ml[(2 * obuf + 1) * kTile + row];
       }
+      // The last read of O: the products of a next item may overwrite it.
+      auto release = [&]() {
+        if (!any) return;
+        tc_fence_before();
+        mbar_arrive(&o_empty[obuf]);
+        ++busy;
+      };
       if (items.splits > 1) {
         const int64_t at2 = live ? (row_index(a, b, i, h) * items.splits + split) * 2 : 0;
         if (live) a.part_ml[at2] = v0, a.part_ml[at2 + 1] = v1;
         if (any) {
 #pragma unroll 1
-          for (int c = 0; c < 2 * static_cast<int>(G::kDv) / 16; ++c) {  // O of map 0, then of map 1
-            uint32_t o[16];
-            tmem_ld16(o_addr + 16 * c, o);
+          for (int c = 0; c < 2 * static_cast<int>(G::kDv) / 32; ++c) {  // O of map 0, then of map 1
+            uint32_t o[32];
+            tmem_ld32(o_addr + 32 * c, o);
             tmem_ld_wait(o);
             if (live) {
-              float4* dst = reinterpret_cast<float4*>(a.part_o + at2 * G::kDv + 16 * c);
+              float4* dst = reinterpret_cast<float4*>(a.part_o + at2 * G::kDv + 32 * c);
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
+              for (int k = 0; k < 8; ++k)
                 dst[k] = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]),
                                      __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
             }
           }
         }
-      } else {
-        const float w0 = v0.y == 0.0f ? 0.0f : 1.0f / v0.y;
-        const float w1 = v1.y == 0.0f ? 0.0f : a.lambda[h] / v1.y;
-        uint16_t* out = a.out + b * a.d.out_batch + i * a.d.out_token + h * a.d.out_head;
-        // Two passes over O in tensor memory: the sum of squares, the output.
-        float f = a.d.out_scale;
-        if (any && a.gamma) {
-          float ss = 0.0f;
-#pragma unroll 1
-          for (int c = 0; c < static_cast<int>(G::kDv) / 16; ++c) {
-            uint32_t o0[16], o1[16];
-            tmem_ld16(o_addr + 16 * c, o0);
-            tmem_ld16(o_addr + G::kDv + 16 * c, o1);
-            tmem_ld_wait(o0);
-            tmem_ld_wait(o1);
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              const float r = __uint_as_float(o0[k]) * w0 - __uint_as_float(o1[k]) * w1;
-              ss = fmaf(r, r, ss);
-            }
-          }
-          f *= 1.0f / sqrtf(ss / static_cast<float>(G::kDv) + a.d.eps);
-        }
-#pragma unroll 1
-        for (int c = 0; c < static_cast<int>(G::kDv) / 16; ++c) {
-          uint32_t o0[16], o1[16], w[8];
-          if (any) {
-            tmem_ld16(o_addr + 16 * c, o0);
-            tmem_ld16(o_addr + G::kDv + 16 * c, o1);
-            tmem_ld_wait(o0);
-            tmem_ld_wait(o1);
-          }
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            float2 r = make_float2(0.0f, 0.0f);
-            if (any) {
-              r.x = (__uint_as_float(o0[2 * k]) * w0 - __uint_as_float(o1[2 * k]) * w1) * f;
-              r.y = (__uint_as_float(o0[2 * k + 1]) * w0 - __uint_as_float(o1[2 * k + 1]) * w1) * f;
-              if (a.gamma) r.x *= a.gamma[16 * c + 2 * k], r.y *= a.gamma[16 * c + 2 * k + 1];
-            }
-            w[k] = pack16x2(r, F16);
-          }
-          if (live) {
-            *reinterpret_cast<uint4*>(out + 16 * c) = make_uint4(w[0], w[1], w[2], w[3]);
-            *reinterpret_cast<uint4*>(out + 16 * c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
-          }
-        }
+        release();
+        continue;
       }
-      if (any) {
-        tc_fence_before();
-        mbar_arrive(o_empty);
-        ++busy;
+      const float w0 = v0.y == 0.0f ? 0.0f : 1.0f / v0.y;
+      const float w1 = v1.y == 0.0f ? 0.0f : lambda / v1.y;
+      uint16_t* out = a.out + b * a.d.out_batch + i * a.d.out_token + h * a.d.out_head;
+      constexpr int kChunks = static_cast<int>(G::kDv) / 32;
+      // 32 dims of the difference.
+      auto difference = [&](int c, float2 (&r)[16]) {
+        if (!any) {
+#pragma unroll
+          for (int k = 0; k < 16; ++k) r[k] = make_float2(0.0f, 0.0f);
+          return;
+        }
+        uint32_t o0[32], o1[32];
+        tmem_ld32(o_addr + 32 * c, o0);
+        tmem_ld32(o_addr + G::kDv + 32 * c, o1);
+        tmem_ld_wait(o0);
+        tmem_ld_wait(o1);
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+          r[k] = fma2(make_float2(__uint_as_float(o0[2 * k]), __uint_as_float(o0[2 * k + 1])), make_float2(w0, w0),
+                      mul2(make_float2(__uint_as_float(o1[2 * k]), __uint_as_float(o1[2 * k + 1])), make_float2(-w1, -w1)));
+      };
+      // Two passes over O in tensor memory: the sum of squares, the output.
+      float f = a.d.out_scale;
+      float2 r[16];
+      if (a.gamma) {
+        float2 ss = make_float2(0.0f, 0.0f);
+#pragma unroll 1
+        for (int c = 0; c < kChunks; ++c) {
+          difference(c, r);
+#pragma unroll
+          for (int k = 0; k < 16; ++k) ss = fma2(r[k], r[k], ss);
+        }
+        f *= rsqrtf((ss.x + ss.y) / static_cast<float>(G::kDv) + a.d.eps);
+      }
+#pragma unroll 1
+      for (int c = 0; c < kChunks; ++c) {
+        difference(c, r);
+        if (c == kChunks - 1) release();
+        uint32_t w[16];
+#pragma unroll
+        for (int k = 0; k < 16; k += 2) {
+          float4 g = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+          if (a.gamma) g = make_float4(a.gamma[32 * c + 2 * k], a.gamma[32 * c + 2 * k + 1], a.gamma[32 * c + 2 * k + 2], a.gamma[32 * c + 2 * k + 3]);
+          w[k] = pack16x2(make_float2(r[k].x * f * g.x, r[k].y * f * g.y), F16);
+          w[k + 1] = pack16x2(make_float2(r[k + 1].x * f * g.z, r[k + 1].y * f * g.w), F16);
+        }
+        if (live) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            *reinterpret_cast<uint4*>(out + 32 * c + 8 * k) = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+        }
       }
     }
   } else {
@@ -509,15 +540,18 @@ __global__ void __launch_bounds__(kThreads, 1) diff_tc_kernel(const __grid_const
         const int stage = wp.tile % kS;
         const uint64_t vdesc = sw128_mn_desc(smem_u32(smem + G::kVOff + stage * G::kV), G::kVCol);
         if (map == 0 && (!KB_WARP_WAIT(&v_ready[stage], (wp.tile / kS) & 1) ||
-                         (wp.begins_item() && wp.item > 0 && !KB_WARP_WAIT(o_empty, (wp.item - 1) & 1))))
+                         (wp.begins_item() && wp.item >= G::kOBufs &&
+                          !KB_WARP_WAIT(&o_empty[wp.item % G::kOBufs], (wp.item / G::kOBufs - 1) & 1))))
           return false;
+        const int obuf = wp.item % G::kOBufs;
+        const uint32_t o_tmem = tmem + G::kO + (2 * obuf + map) * G::kDv;
         const uint32_t add = !wp.begins_item();
         if (!KB_WARP_WAIT(&p_full[2 * map], wp.tile & 1)) return false;
         tc_fence_after();
         if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < kFirst / 16; ++k)
-            mma_f16_ts(tmem + G::kO + map * G::kDv, tmem + map * 128 + 8 * k,
+            mma_f16_ts(o_tmem, tmem + map * 128 + 8 * k,
                        vdesc + static_cast<uint64_t>(k * 16 * 128 >> 4), kIdV, k == 0 ? add : 1u);
         }
         __syncwarp();
@@ -526,10 +560,10 @@ __global__ void __launch_bounds__(kThreads, 1) diff_tc_kernel(const __grid_const
         if (elect_one()) {
 #pragma unroll
           for (int k = kFirst / 16; k < kTile / 16; ++k)
-            mma_f16_ts(tmem + G::kO + map * G::kDv, tmem + map * 128 + 8 * k,
+            mma_f16_ts(o_tmem, tmem + map * 128 + 8 * k,
                        vdesc + static_cast<uint64_t>(k * 16 * 128 >> 4), kIdV, 1u);
           tc_commit(&pv_done[map]);
-          if (wp.ends_item()) tc_commit(&o_full[map]);
+          if (wp.ends_item()) tc_commit(&o_full[2 * obuf + map]);
           if (map == 1) tc_commit(&v_empty[stage]);
         }
         __syncwarp();
@@ -616,9 +650,13 @@ __global__ void __launch_bounds__(kThreads, 1) diff_tc_kernel(const __grid_const
             const int key = t * kTile + 32 * c + lane;
             see[c] = __ballot_sync(0xffffffffu, key < n && (!has_mask || mask[key] != 0));
           }
+          const bool all = (see[0] & see[1] & see[2] & see[3]) == 0xffffffffu;
           if (has_mask) {
-            if (lane < 4) mask_bits[stage * 4 + lane] = lane == 0 ? see[0] : lane == 1 ? see[1] : lane == 2 ? see[2] : see[3];
-            mbar_arrive(&bits_full[stage]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              limits[stage * kTile + 32 * c + lane] = see[c] >> lane & 1u ? INFINITY : -INFINITY;
+            if (lane == 0) all_seen[stage] = all;
+            mbar_arrive(&limit_full[stage]);
           }
           if (!KB_WARP_WAIT(&v_full[stage], parity)) {
             ok = false;
@@ -627,7 +665,7 @@ __global__ void __launch_bounds__(kThreads, 1) diff_tc_kernel(const __grid_const
           uint8_t* v = smem + G::kVOff + stage * G::kV;
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            if (see[c] == 0xffffffffu) continue;
+            if (all || see[c] == 0xffffffffu) continue;
             // four rows at a time, 8 lanes a row; swizzling stays within a row
             for (int r = lane >> 3; r < 32; r += 4)
               if (!(see[c] >> r & 1u))
@@ -706,11 +744,14 @@ int launch(const DiffArgs& a, int splits, unsigned* status, cudaStream_t s) {
   it.q_tiles = (d.q_len + kTile - 1) / kTile;
   it.splits = splits;
   const int64_t count = static_cast<int64_t>(d.batch) * d.heads * it.q_tiles * splits;
-  if (count > 0x7fffffff - 1024) {
+  if (count > 0x7fffffff - 65536 || static_cast<int64_t>(d.batch) * d.heads > 0x3fffffff) {
     set_error("kb_diff_attention: too many query tiles");
     return KB_E_INVALID;
   }
   it.count = static_cast<int>(count);
+  it.by_splits = FastDiv(splits);
+  it.by_tiles = FastDiv(d.causal ? d.batch * d.heads : it.q_tiles);
+  it.by_heads = FastDiv(d.heads);
   const int grid = it.count < num_sms(dev) ? it.count : num_sms(dev);
   kern<<<grid, kThreads, Geo<D>::kBytes, s>>>(mq, mk, mv, a, it, bc, status);
   return check_cuda(cudaGetLastError(), "differential attention launch");
