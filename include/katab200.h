@@ -331,16 +331,18 @@ KB_API int kb_norm_residual(const kb_norm_residual_desc* desc, const void* x, co
  * the last `window` of them.  A query that sees no key gets zeros.  What lies
  * in K and V at keys that kv_lens or key_mask hide is never used, NaN and
  * infinities included; a non-finite value of V at a key that only the causal
- * mask or the window hides may reach other queries of the call. */
+ * mask or the window hides may reach other queries of the call.
+ * At most 2^26 queries and keys, 1024 heads and 65535 sequences. */
 typedef struct kb_diff_attention_desc {
   int dtype;           /* KB_DT_F16 or KB_DT_BF16 */
   int batch, q_len, kv_len;
   int heads, kv_heads; /* heads a multiple of kv_heads */
   int head_dim;        /* 32 or 64: of each map; values and outputs are twice as wide */
   int causal, window;  /* window 0: none; needs causal */
-  float scale, out_scale, eps;
-  /* strides in elements, multiples of 8 (dimensions of extent 1: ignored); the
-   * base addresses are 16-byte aligned */
+  float scale, out_scale, eps; /* scale > 0 */
+  /* strides in elements, multiples of 8 (dimensions of extent 1: ignored); 0
+   * broadcasts q, k or v over sequences, heads or maps; the base addresses are
+   * 16-byte aligned */
   int64_t q_batch, q_token, q_head, q_map;
   int64_t k_batch, k_token, k_head, k_map;
   int64_t v_batch, v_token, v_head;

@@ -30,7 +30,7 @@ import numpy as np
 import torch
 
 from . import _capi
-from ._capi import call
+from ._capi import call, check, load
 
 _DTYPES = {torch.float32: _capi.DT_F32, torch.float16: _capi.DT_F16, torch.bfloat16: _capi.DT_BF16}
 _LAYOUTS = {"pairs": _capi.ROPE_PAIRS, "halves": _capi.ROPE_HALVES}
@@ -80,6 +80,9 @@ def _device(t, what):
 
 def _check(t, what, shape, dtype, device):
     """The address of `t`; raises unless it has this shape, type and device and a contiguous last dimension."""
+    if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == device
+            and (t.stride(-1) == 1 or shape[-1] < 2)):
+        return t.data_ptr()
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{what} must be a tensor")
     if t.dtype is not dtype:
@@ -88,9 +91,13 @@ def _check(t, what, shape, dtype, device):
         raise ValueError(f"{what} must be on device {device}, got {t.device}")
     if t.shape != shape:
         raise ValueError(f"{what} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
-        raise ValueError(f"{what}'s last dimension must be contiguous")
-    return t.data_ptr()
+    raise ValueError(f"{what}'s last dimension must be contiguous")
+
+
+@functools.cache
+def _native(name):
+    """A function of the library (loaded at the first call), without the lookups of a call by name."""
+    return getattr(load(), name)
 
 
 def _on(stream, device):
@@ -102,7 +109,7 @@ def _on(stream, device):
 
 def _empty(like, shape, dtype, stream, device):
     if stream is None:
-        return like.new_empty(shape, dtype=dtype)
+        return like.new_empty(shape) if like.dtype is dtype else like.new_empty(shape, dtype=dtype)
     with _on(stream, device):
         return like.new_empty(shape, dtype=dtype)
 
@@ -117,16 +124,16 @@ def rope_axes(x, positions, freqs, out=None, *, rotary_heads=None, layout="pairs
     heads, head_dim] (a cache), rows outside it are skipped.  Returns out.
     """
     device = _device(x, "x")
-    dtype = x.dtype
+    dtype, shape = x.dtype, x.shape
     kind = _lookup(_DTYPES, dtype, "x's dtype")
-    if x.dim() != 3 or freqs.dim() != 3:
+    if len(shape) != 3 or freqs.dim() != 3:
         raise ValueError("x must be [tokens, heads, head_dim] and freqs [heads, pairs, axes]")
-    shape = x.shape
     tokens, heads, head_dim = shape
-    freq_heads, pairs, axes = freqs.shape
+    freq_shape = freqs.shape
+    freq_heads, pairs, axes = freq_shape
     xp = _check(x, "x", shape, dtype, device)
     pp = _check(positions, "positions", (axes, tokens), torch.int32, device)
-    fp = _check(freqs, "freqs", (freq_heads, pairs, axes), torch.float32, device)
+    fp = _check(freqs, "freqs", freq_shape, torch.float32, device)
     if not positions.is_contiguous() or not freqs.is_contiguous():
         raise ValueError("positions and freqs must be contiguous")
     sp = rows = 0
@@ -141,9 +148,12 @@ def rope_axes(x, positions, freqs, out=None, *, rotary_heads=None, layout="pairs
         if slots is not None:
             sp = _check(slots, "slots", (tokens,), torch.int64, device)
     xs, os = x.stride(), out.stride()
-    call("kb_rope_axes", xp, kind, tokens, heads, head_dim, xs[0], xs[1], pp, axes, fp, freq_heads, pairs,
-         heads if rotary_heads is None else rotary_heads, _lookup(_LAYOUTS, layout, "layout"), sp, rows, op, os[0],
-         os[1], _raw(stream, device))
+    code = _native("kb_rope_axes")(
+        xp, kind, tokens, heads, head_dim, xs[0], xs[1], pp, axes, fp, freq_heads, pairs,
+        heads if rotary_heads is None else rotary_heads, _lookup(_LAYOUTS, layout, "layout"), sp, rows, op, os[0],
+        os[1], _raw(stream, device))
+    if code:
+        check(code)
     return out
 
 
@@ -180,9 +190,11 @@ def norm_residual(x, y=None, *, post=None, pre=None, post_gamma=None, post_beta=
     branch_kind = _lookup(_DTYPES, h_dtype, "h's dtype")
     if rows_per_cond < 1:
         raise ValueError("rows_per_cond must be positive")
-    affine = [0 if t is None else _check(t, what, (width,), torch.float32, device)
-              for t, what in ((post_gamma, "post_gamma"), (post_beta, "post_beta"), (pre_gamma, "pre_gamma"),
-                              (pre_beta, "pre_beta"))]
+    row, f32 = (width,), torch.float32
+    affine = (0 if post_gamma is None else _check(post_gamma, "post_gamma", row, f32, device),
+              0 if post_beta is None else _check(post_beta, "post_beta", row, f32, device),
+              0 if pre_gamma is None else _check(pre_gamma, "pre_gamma", row, f32, device),
+              0 if pre_beta is None else _check(pre_beta, "pre_beta", row, f32, device))
     cond, cond_stride = (0, 0, 0), None
     if gate is not None or mod_scale is not None or mod_shift is not None:
         cond = []
@@ -215,7 +227,9 @@ def norm_residual(x, y=None, *, post=None, pre=None, post_gamma=None, post_beta=
         rows, width, stream_kind, branch_kind, _lookup(_NORMS, post, "post"), _lookup(_NORMS, pre, "pre"),
         _lookup(_GATES, gate_act, "gate_act"), rows_per_cond, res_scale, branch_scale, eps, x_stride, y_stride,
         xo_stride, h_stride, cond_stride or 0)
-    call("kb_norm_residual", desc, xp, yp, *affine, *cond, xo_p, h_p, _raw(stream, device))
+    code = _native("kb_norm_residual")(desc, xp, yp, *affine, *cond, xo_p, h_p, _raw(stream, device))
+    if code:
+        check(code)
     return x_out, h
 
 
@@ -243,11 +257,12 @@ def diff_attention(q, k, v, lam, *, gamma=None, out_scale=1.0, eps=1e-5, scale=N
     dtype = q.dtype
     if dtype is not torch.bfloat16 and dtype is not torch.float16:
         raise TypeError(f"q must be float16 or bfloat16, got {dtype}")
-    if q.dim() != 5 or k.dim() != 5:
+    q_shape, k_shape = q.shape, k.shape
+    if len(q_shape) != 5 or len(k_shape) != 5 or q_shape[3] != 2:
         raise ValueError("q and k must be [batch, tokens, heads, 2, d]")
-    batch, q_len, heads, _, d = q.shape
-    _, kv_len, kv_heads, _, _ = k.shape
-    qp = _check(q, "q", (batch, q_len, heads, 2, d), dtype, device)
+    batch, q_len, heads, _, d = q_shape
+    kv_len, kv_heads = k_shape[1], k_shape[2]
+    qp = _check(q, "q", q_shape, dtype, device)
     kp = _check(k, "k", (batch, kv_len, kv_heads, 2, d), dtype, device)
     vp = _check(v, "v", (batch, kv_len, kv_heads, 2 * d), dtype, device)
     lp = _check(lam, "lam", (heads,), torch.float32, device)
@@ -263,16 +278,19 @@ def diff_attention(q, k, v, lam, *, gamma=None, out_scale=1.0, eps=1e-5, scale=N
         op = out.data_ptr()
     else:
         op = _check(out, "out", (batch, q_len, heads, 2 * d), dtype, device)
+    qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
     desc = _DIFF_DESC.pack(
         _DTYPES[dtype], batch, q_len, kv_len, heads, kv_heads, d, bool(causal), window,
-        d**-0.5 if scale is None else scale, out_scale, eps, *q.stride()[:4], *k.stride()[:4], *v.stride()[:3],
-        *out.stride()[:3], mask_batch)
+        d**-0.5 if scale is None else scale, out_scale, eps, qs[0], qs[1], qs[2], qs[3], ks[0], ks[1], ks[2], ks[3],
+        vs[0], vs[1], vs[2], os[0], os[1], os[2], mask_batch)
     need, wp = _workspace_bytes(desc, device), 0
     if need:
         work = _empty(q, need, torch.uint8, stream, device)
         wp = work.data_ptr()
-    call("kb_diff_attention", desc, qp, kp, vp, lp, gp, np_, mp, op, wp, need,
-         0 if status is None else status.data_ptr(), _raw(stream, device))
+    code = _native("kb_diff_attention")(desc, qp, kp, vp, lp, gp, np_, mp, op, wp, need,
+                                        0 if status is None else status.data_ptr(), _raw(stream, device))
+    if code:
+        check(code)
     return out
 
 

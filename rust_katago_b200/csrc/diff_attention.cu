@@ -146,8 +146,9 @@ int check_desc(const kb_diff_attention_desc* desc) {
   if (d.dtype != KB_DT_F16 && d.dtype != KB_DT_BF16) return bad("dtype must be KB_DT_F16 or KB_DT_BF16");
   if (d.head_dim != 32 && d.head_dim != 64) return bad("head_dim must be 32 or 64");
   if (d.batch < 0 || d.q_len < 0 || d.kv_len < 0) return bad("batch, q_len and kv_len must not be negative");
-  if (d.batch > 65535 || d.q_len > (1 << 26) || d.kv_len > (1 << 30) || d.heads > 1024)
-    return bad("at most 65535 sequences, 2^26 queries, 2^30 keys and 1024 heads");
+  // (2^26 keys take a block about a second, below the limit of the kernels' waits.)
+  if (d.batch > 65535 || d.q_len > (1 << 26) || d.kv_len > (1 << 26) || d.heads > 1024)
+    return bad("at most 65535 sequences, 2^26 queries, 2^26 keys and 1024 heads");
   if (d.heads < 1 || d.kv_heads < 1 || d.heads % d.kv_heads) return bad("heads must be a multiple of kv_heads");
   if (d.window < 0 || (d.window > 0 && !d.causal)) return bad("a window must be positive and causal");
   if (!(d.scale > 0.0f) || !isfinite(d.scale) || !isfinite(d.out_scale) || !(d.eps >= 0.0f))

@@ -31,6 +31,7 @@ inline DiffArgs make_diff_args(const kb_diff_attention_desc& desc, const uint16_
   DiffArgs a{desc, q, k, v, lambda, gamma, kv_lens, key_mask, out, desc.scale * 1.4426950408889634f,
              nullptr, nullptr};
   kb_diff_attention_desc& d = a.d;
+  if (d.window >= d.kv_len) d.window = 0;  // hides nothing (and would overflow positions)
   if (d.batch == 1) d.q_batch = d.k_batch = d.v_batch = d.out_batch = d.mask_batch = 0;
   if (d.q_len == 1) d.q_token = d.out_token = 0;
   if (d.kv_len <= 1) d.k_token = d.v_token = 0;

@@ -44,12 +44,21 @@ struct Raw8 {
   uint4 w[DT == KB_DT_F32 ? 2 : 1];
 };
 
+// A load that the compiler may move across the stores of other rows (which it
+// cannot know to be other addresses), but not through the read-only path:
+// outputs may be inputs.
+__device__ __forceinline__ uint4 load_row16(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
 template <int DT>
 __device__ __forceinline__ Raw8<DT> load8(const void* p, int64_t at) {
   Raw8<DT> r;
   const uint4* q = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) + at * (DT == KB_DT_F32 ? 4 : 2));
-  r.w[0] = __ldg(q);
-  if constexpr (DT == KB_DT_F32) r.w[1] = __ldg(q + 1);
+  r.w[0] = load_row16(q);
+  if constexpr (DT == KB_DT_F32) r.w[1] = load_row16(q + 1);
   return r;
 }
 

@@ -425,6 +425,14 @@ def test_offsets_past_32_bits(cuda, q_len):
     assert torch.equal(block.diff_attention(q, kf, vf, lam, **kw), block.diff_attention(q, k, v, lam, **kw))
 
 
+def test_window_wider_than_the_keys_hides_nothing(cuda):
+    for q_len, kv_len in ((1, 300), (140, 140)):
+        q, k, v, lam, gamma = attn_inputs(1, q_len, kv_len, 2, 2, 64, torch.bfloat16)
+        ref = block.diff_attention(q, k, v, lam, gamma=gamma, causal=True)
+        for window in (kv_len, 2**31 - 1):
+            assert torch.equal(block.diff_attention(q, k, v, lam, gamma=gamma, causal=True, window=window), ref)
+
+
 def test_empty_lengths(cuda):
     q, k, v, lam, gamma = attn_inputs(2, 5, 8, 2, 2, 64, torch.bfloat16)
     got = block.diff_attention(q, k[:, :0], v[:, :0], lam, gamma=gamma)
