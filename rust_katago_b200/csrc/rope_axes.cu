@@ -97,10 +97,16 @@ __device__ __forceinline__ typename Raw<T, VE>::type pack(const float (&v)[VE], 
   return raw;
 }
 
-template <typename R>
-__device__ __forceinline__ R load(const R* p) {  // streamed: in place, nothing else reads it
-  return __ldcs(p);
+// Loads that stay where they are written, ahead of the work on the tokens before
+// (the compiler otherwise moves them to their first use), and that see what an
+// in-place call has written.
+__device__ __forceinline__ uint4 load(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
 }
+__device__ __forceinline__ uint16_t load(const uint16_t* p) { return *p; }
+__device__ __forceinline__ float load(const float* p) { return *p; }
 
 // A thread's item: 2 VE elements of one head, VE of them at o0 and VE at o1.
 // KB_ROPE_HALVES: u at o0 and v at o1 for pairs o0..; KB_ROPE_PAIRS: the pairs
