@@ -18,6 +18,7 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "kb_internal.h"
 #include "kb_numeric.cuh"
@@ -37,7 +38,11 @@ struct NormArgs {
 // leave little idle.
 constexpr int kRunsPerSlot = 2;
 constexpr int kResident1 = 20, kResident2 = 20;
-// ------------------------------------------------------------------ whole groups of eight columns
+// ------------------------------------------------------------------ typed kernels
+// A thread holds NC chunks of eight columns.  VEC: chunk c is columns 8 (c TPR +
+// i).. of the row, 16 or 32 bytes an access; otherwise element e of chunk c is
+// column (8 c + e) TPR + i, an element an access, for rows of any width and
+// alignment.
 // Eight columns of type DT as fp32 pairs, and back.
 template <int DT>
 struct Raw8 {
@@ -60,6 +65,34 @@ __device__ __forceinline__ Raw8<DT> load8(const void* p, int64_t at) {
   r.w[0] = load_row16(q);
   if constexpr (DT == KB_DT_F32) r.w[1] = load_row16(q + 1);
   return r;
+}
+
+// Eight single elements.
+template <int DT>
+struct Raw1 {
+  std::conditional_t<DT == KB_DT_F32, float, uint16_t> e[8];
+};
+
+template <int DT>
+__device__ __forceinline__ void load_one(const void* p, int64_t at, bool in, Raw1<DT>& r, int e) {
+  if constexpr (DT == KB_DT_F32) {
+    float v = 0.0f;
+    if (in) asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(static_cast<const float*>(p) + at));
+    r.e[e] = v;
+  } else {
+    uint16_t v = 0;
+    if (in) asm volatile("ld.global.u16 %0, [%1];" : "=h"(v) : "l"(static_cast<const uint16_t*>(p) + at));
+    r.e[e] = v;
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ void open8(const Raw1<DT>& r, float2 (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (DT == KB_DT_F32) v[i] = make_float2(r.e[2 * i], r.e[2 * i + 1]);
+    else v[i] = make_float2(from16(r.e[2 * i], DT == KB_DT_F16), from16(r.e[2 * i + 1], DT == KB_DT_F16));
+  }
 }
 
 template <int DT>
@@ -115,9 +148,9 @@ __device__ __forceinline__ float group_sum(float2 v, float (*red)[16], int& turn
 }
 
 // v -> v centred (KB_NORM_LAYER); returns the factor 1 / sqrt(mean(v^2) + eps),
-// or 1 without a norm.  Chunks outside the row hold zeros.
-template <int NC, bool BLOCK>
-__device__ __forceinline__ float normalise(float2 (&v)[NC][4], int kind, float inv_width, float eps, int valid,
+// or 1 without a norm.  Columns outside the row hold zeros.
+template <int NC, bool BLOCK, bool VEC, typename In>
+__device__ __forceinline__ float normalise(float2 (&v)[NC][4], int kind, float inv_width, float eps, const In& in,
                                            float (*red)[16], int& turn) {
   if (kind == KB_NORM_NONE) return 1.0f;
   if (kind == KB_NORM_LAYER) {
@@ -128,10 +161,14 @@ __device__ __forceinline__ float normalise(float2 (&v)[NC][4], int kind, float i
       for (int i = 0; i < 4; ++i) s = add2(s, v[c][i]);
     const float mean = group_sum<BLOCK>(s, red, turn) * inv_width;
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
-      if (c < valid)
+    for (int c = 0; c < NC; ++c) {
+      if (VEC && !in(c, 0)) continue;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[c][i] = add2(v[c][i], both(-mean));
+      for (int i = 0; i < 4; ++i) {
+        v[c][i] = add2(v[c][i], both(-mean));
+        if constexpr (!VEC) v[c][i] = make_float2(in(c, 2 * i) ? v[c][i].x : 0.0f, in(c, 2 * i + 1) ? v[c][i].y : 0.0f);
+      }
+    }
   }
   float2 s0 = both(0.0f), s1 = both(0.0f);
 #pragma unroll
@@ -152,7 +189,7 @@ __device__ __forceinline__ float gate_value(float v, int act) {
 
 // XT, YT: types of stream and branch.  SHIFT: 0 no shifts, 1 only B, 2 also C.
 // THREADS: 32 (a warp per row) or the most that a block has.
-template <int XT, int YT, int NC, int THREADS, int SHIFT>
+template <int XT, int YT, int NC, int THREADS, int SHIFT, bool VEC>
 __global__ void __launch_bounds__(THREADS, THREADS == 320 ? 2 : 1) norm_rows_kernel(const NormArgs a,
                                                                                    int rows_per_group) {
   constexpr bool BLOCK = THREADS > 32;
@@ -169,9 +206,41 @@ __global__ void __launch_bounds__(THREADS, THREADS == 320 ? 2 : 1) norm_rows_ker
   const int64_t end = min(row + rows_per_group, static_cast<int64_t>(d.rows));
   if (row >= end) return;
   const int col = i * 8, step = tpr * 8;
-  int valid = 0;  // chunks of this thread inside the row
+  int valid = 0;  // VEC: chunks of this thread inside the row
 #pragma unroll
   for (int c = 0; c < NC; ++c) valid += col + c * step < d.width;
+  auto column = [&](int c, int e) { return VEC ? col + c * step + e : (c * 8 + e) * tpr + i; };
+  auto inside = [&](int c, int e) { return VEC ? c < valid : column(c, e) < d.width; };
+  // Eight columns of a tensor of type DT at element `row_at` (VEC: of a chunk
+  // inside the row; otherwise with zeros outside it).
+  auto get = [&](auto dt, const void* p, int64_t row_at, int c) {
+    constexpr int DT = decltype(dt)::value;
+    if constexpr (VEC) {
+      return load8<DT>(p, row_at + column(c, 0));
+    } else {
+      Raw1<DT> r;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) load_one<DT>(p, row_at + column(c, e), inside(c, e), r, e);
+      return r;
+    }
+  };
+  auto put = [&](auto dt, void* p, int64_t row_at, int c, const float2 (&v)[4]) {
+    constexpr int DT = decltype(dt)::value;
+    if constexpr (VEC) {
+      if (c < valid) store8<DT>(p, row_at + column(c, 0), v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (!inside(c, e)) continue;
+        const float f = e & 1 ? v[e / 2].y : v[e / 2].x;
+        if constexpr (DT == KB_DT_F32) static_cast<float*>(p)[row_at + column(c, e)] = f;
+        else static_cast<uint16_t*>(p)[row_at + column(c, e)] = bits16(f, DT == KB_DT_F16);
+      }
+    }
+  };
+  constexpr std::integral_constant<int, KB_DT_F32> kF32{};
+  constexpr std::integral_constant<int, XT> kX{};
+  constexpr std::integral_constant<int, YT> kY{};
   const float inv_width = 1.0f / static_cast<float>(d.width);
   int turn = 0;
 
@@ -192,17 +261,15 @@ __global__ void __launch_bounds__(THREADS, THREADS == 320 ? 2 : 1) norm_rows_ker
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       float2 gv[4], av[4], cv[4], bv[4];
-      const int at = col + c * step;
       float2 t[4], u[4];
-      const bool in = c < valid;
       auto param = [&](const float* p, float otherwise, float2 (&v)[4]) {
-        if (p && in) open8<KB_DT_F32>(load8<KB_DT_F32>(p, at), v);
+        if (p && (!VEC || c < valid)) open8(get(kF32, p, 0, c), v);
         else
 #pragma unroll
           for (int k = 0; k < 4; ++k) v[k] = both(otherwise);
       };
       auto mod = [&](const void* p, float otherwise, float2 (&v)[4]) {
-        if (p && in) open8<YT>(load8<YT>(p, cond * d.cond_stride + at), v);
+        if (p && (!VEC || c < valid)) open8(get(kY, p, cond * d.cond_stride, c), v);
         else
 #pragma unroll
           for (int k = 0; k < 4; ++k) v[k] = both(otherwise);
@@ -240,21 +307,18 @@ __global__ void __launch_bounds__(THREADS, THREADS == 320 ? 2 : 1) norm_rows_ker
     }
   };
 
-  Raw8<XT> xr[NC];
-  Raw8<YT> yr[NC];
+  std::conditional_t<VEC, Raw8<XT>, Raw1<XT>> xr[NC];
+  std::conditional_t<VEC, Raw8<YT>, Raw1<YT>> yr[NC];
   auto fetch = [&](int64_t at) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      if (c >= valid) continue;
-      xr[c] = load8<XT>(a.x, at * d.x_stride + col + c * step);
-      if (a.y) yr[c] = load8<YT>(a.y, at * d.y_stride + col + c * step);
+      if (VEC && c >= valid) continue;  // stays zero
+      xr[c] = get(kX, a.x, at * d.x_stride, c);
+      if (a.y) yr[c] = get(kY, a.y, at * d.y_stride, c);
     }
   };
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    xr[c] = Raw8<XT>{};
-    yr[c] = Raw8<YT>{};
-  }
+  for (int c = 0; c < NC; ++c) xr[c] = {}, yr[c] = {};
   fetch(row);
   const bool conditioned = a.gate || a.mod_scale || a.mod_shift;
   int64_t cond = conditioned ? row / d.rows_per_cond : 0, next_cond = conditioned ? (cond + 1) * d.rows_per_cond : end;
@@ -267,12 +331,12 @@ __global__ void __launch_bounds__(THREADS, THREADS == 320 ? 2 : 1) norm_rows_ker
     float2 r[NC][4], n[NC][4];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      open8<XT>(xr[c], r[c]);
-      open8<YT>(yr[c], n[c]);
+      open8(xr[c], r[c]);
+      open8(yr[c], n[c]);
     }
     if (row + 1 < end) fetch(row + 1);
     if (a.y) {
-      const float2 f = both(normalise<NC, BLOCK>(n, d.post_norm, inv_width, d.eps, valid, red, turn));
+      const float2 f = both(normalise<NC, BLOCK, VEC>(n, d.post_norm, inv_width, d.eps, inside, red, turn));
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         float2 gv[4], cv[4];
@@ -294,13 +358,12 @@ __global__ void __launch_bounds__(THREADS, THREADS == 320 ? 2 : 1) norm_rows_ker
     }
     if (a.x_out)
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
-        if (c < valid) store8<XT>(a.x_out, row * d.x_out_stride + col + c * step, r[c]);
+      for (int c = 0; c < NC; ++c) put(kX, a.x_out, row * d.x_out_stride, c, r[c]);
     if (a.h) {
-      const float2 f = both(normalise<NC, BLOCK>(r, d.pre_norm, inv_width, d.eps, valid, red, turn));
+      const float2 f = both(normalise<NC, BLOCK, VEC>(r, d.pre_norm, inv_width, d.eps, inside, red, turn));
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        if (c >= valid) continue;
+        if (VEC && c >= valid) continue;
         float2 av[4], bv[4];
         vector(1, c, av);
         if constexpr (SHIFT) vector(2, c, bv);
@@ -310,7 +373,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 320 ? 2 : 1) norm_rows_ker
           if constexpr (SHIFT) r[c][k] = fma2(t, av[k], bv[k]);
           else r[c][k] = mul2(t, av[k]);
         }
-        store8<YT>(a.h, row * d.h_stride + col + c * step, r[c]);
+        put(kY, a.h, row * d.h_stride, c, r[c]);
       }
     }
   }
@@ -320,14 +383,14 @@ __global__ void __launch_bounds__(THREADS, THREADS == 320 ? 2 : 1) norm_rows_ker
 // packs best at 90 to 190 registers a thread), wider ones a block of threads
 // with 16 columns each; enough groups to fill the SMs, each with a run of
 // neighbouring rows.
-template <int XT, int YT, int NC, int THREADS, int SHIFT>
+template <int XT, int YT, int NC, int THREADS, int SHIFT, bool VEC>
 int launch_shift(const NormArgs& a, cudaStream_t s) {
-  auto kern = norm_rows_kernel<XT, YT, NC, THREADS, SHIFT>;
+  auto kern = norm_rows_kernel<XT, YT, NC, THREADS, SHIFT, VEC>;
   int dev = 0;
   cudaGetDevice(&dev);
   int threads = 32, resident = NC == 1 ? kResident1 : NC == 2 ? kResident2 : 16;
   if (THREADS > 32) {
-    threads = (a.d.width / 8 + NC * 32 - 1) / (NC * 32) * 32;
+    threads = ((a.d.width + 7) / 8 + NC * 32 - 1) / (NC * 32) * 32;
     resident = THREADS == 320 ? 2 : 1;
   }
   const int bytes = (2 + SHIFT) * NC * threads * 32;
@@ -350,27 +413,34 @@ int launch_shift(const NormArgs& a, cudaStream_t s) {
   return check_cuda(cudaGetLastError(), "norm launch");
 }
 
-template <int XT, int YT, int NC, int THREADS>
+template <int XT, int YT, int NC, int THREADS, bool VEC>
 int launch_rows(const NormArgs& a, cudaStream_t s) {
-  if (a.post_beta) return launch_shift<XT, YT, NC, THREADS, 2>(a, s);
-  if (a.pre_beta || a.mod_shift) return launch_shift<XT, YT, NC, THREADS, 1>(a, s);
-  return launch_shift<XT, YT, NC, THREADS, 0>(a, s);
+  if constexpr (VEC) {
+    if (!a.post_beta && !a.pre_beta && !a.mod_shift) return launch_shift<XT, YT, NC, THREADS, 0, true>(a, s);
+    if (!a.post_beta) return launch_shift<XT, YT, NC, THREADS, 1, true>(a, s);
+  }
+  return launch_shift<XT, YT, NC, THREADS, 2, VEC>(a, s);
 }
 
 constexpr int kTypedWidth = 8192;  // the widest row of the typed kernels
 
-template <int XT, int YT>
-int launch_typed(const NormArgs& a, cudaStream_t s) {
-  const int chunks = a.d.width / 8;
-  if (chunks <= 32) return launch_rows<XT, YT, 1, 32>(a, s);
-  if (chunks <= 64) return launch_rows<XT, YT, 2, 32>(a, s);
-  if (chunks <= 96) return launch_rows<XT, YT, 3, 32>(a, s);
-  if (chunks <= 128) return launch_rows<XT, YT, 4, 32>(a, s);
-  if (chunks <= 640) return launch_rows<XT, YT, 2, 320>(a, s);
-  return launch_rows<XT, YT, 2, 512>(a, s);
+template <int XT, int YT, bool VEC>
+int launch_width(const NormArgs& a, cudaStream_t s) {
+  const int chunks = (a.d.width + 7) / 8;
+  if (chunks <= 32) return launch_rows<XT, YT, 1, 32, VEC>(a, s);
+  if (chunks <= 64) return launch_rows<XT, YT, 2, 32, VEC>(a, s);
+  if (chunks <= 96) return launch_rows<XT, YT, 3, 32, VEC>(a, s);
+  if (chunks <= 128) return launch_rows<XT, YT, 4, 32, VEC>(a, s);
+  if (chunks <= 640) return launch_rows<XT, YT, 2, 320, VEC>(a, s);
+  return launch_rows<XT, YT, 2, 512, VEC>(a, s);
 }
 
-// ------------------------------------------------------------------ any width and alignment
+template <int XT, int YT>
+int launch_typed(const NormArgs& a, bool vec, cudaStream_t s) {
+  return vec ? launch_width<XT, YT, true>(a, s) : launch_width<XT, YT, false>(a, s);
+}
+
+// ------------------------------------------------------------------ any types and width
 // Values of one row held by one thread: element k is column k TPR + i, one
 // element per access, types chosen at run time.
 
@@ -543,8 +613,8 @@ extern "C" int kb_norm_residual(const kb_norm_residual_desc* desc, const void* x
   if (x_out && x_out == y) return bad("x_out must not be y");
   NormArgs a{d, x, y, post_gamma, post_beta, pre_gamma, pre_beta, gate, mod_scale, mod_shift, x_out, h};
   if (a.d.rows_per_cond < 1) a.d.rows_per_cond = 1;
-  // Eight columns per access need whole groups and 16-byte rows, and the type
-  // pairs that streams have; anything else takes the kernel of single elements.
+  // Eight columns per access need whole groups and 16-byte rows; type pairs that
+  // no stream has and rows above kTypedWidth take the kernel of any types.
   bool vec = d.width % 8 == 0;
   for (const void* p : {x, y, static_cast<const void*>(post_gamma), static_cast<const void*>(post_beta),
                         static_cast<const void*>(pre_gamma), static_cast<const void*>(pre_beta), gate, mod_scale,
@@ -553,13 +623,13 @@ extern "C" int kb_norm_residual(const kb_norm_residual_desc* desc, const void* x
   vec = vec && d.x_stride % 8 == 0 && (!y || d.y_stride % 8 == 0) && (!x_out || d.x_out_stride % 8 == 0) &&
         (!h || d.h_stride % 8 == 0) && (!cond || d.cond_stride % 8 == 0);
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (vec && d.width <= kTypedWidth) {
+  if (d.width <= kTypedWidth) {
     const int x_t = d.stream_dtype, y_t = d.branch_dtype;
-    if (x_t == KB_DT_BF16 && y_t == KB_DT_BF16) return launch_typed<KB_DT_BF16, KB_DT_BF16>(a, s);
-    if (x_t == KB_DT_F16 && y_t == KB_DT_F16) return launch_typed<KB_DT_F16, KB_DT_F16>(a, s);
-    if (x_t == KB_DT_F32 && y_t == KB_DT_BF16) return launch_typed<KB_DT_F32, KB_DT_BF16>(a, s);
-    if (x_t == KB_DT_F32 && y_t == KB_DT_F16) return launch_typed<KB_DT_F32, KB_DT_F16>(a, s);
-    if (x_t == KB_DT_F32 && y_t == KB_DT_F32) return launch_typed<KB_DT_F32, KB_DT_F32>(a, s);
+    if (x_t == KB_DT_BF16 && y_t == KB_DT_BF16) return launch_typed<KB_DT_BF16, KB_DT_BF16>(a, vec, s);
+    if (x_t == KB_DT_F16 && y_t == KB_DT_F16) return launch_typed<KB_DT_F16, KB_DT_F16>(a, vec, s);
+    if (x_t == KB_DT_F32 && y_t == KB_DT_BF16) return launch_typed<KB_DT_F32, KB_DT_BF16>(a, vec, s);
+    if (x_t == KB_DT_F32 && y_t == KB_DT_F16) return launch_typed<KB_DT_F32, KB_DT_F16>(a, vec, s);
+    if (x_t == KB_DT_F32 && y_t == KB_DT_F32) return launch_typed<KB_DT_F32, KB_DT_F32>(a, vec, s);
   }
   return launch_any(a, s);
 }
