@@ -83,8 +83,8 @@ struct Plan {
 };
 
 constexpr int kShortTiles = 36, kShortKeys = 2048;
-constexpr int kFewKeys = 128;  // keys per block of four warps, at least
-constexpr int kClusterKeys = 4096;
+constexpr int kFewKeys = 128;       // keys per block of four warps, at least
+constexpr int kClusterKeys = 4096;  // up to here the join's launch costs more than blocks left idle
 constexpr int kTileKeys = 128;
 constexpr int kTilesPerPart = 4, kMostParts = 32;
 

@@ -13,6 +13,9 @@
 // 2^-32 of a turn, exact for long positions where fp32 is not (position 30,000
 // times a frequency of 1 costs fp32 1e-3).  (In fp64 the conversions bounded
 // the kernel: 92,416 tokens of 36 x 64 bf16 took 195 us.)
+// Measured: that case 162 us, 5.25 TB/s (0.80 of the copy rate), bound by the
+// bytes that 480 threads of 128 registers keep in flight; 32,845 tokens of 12 x 32
+// fp32, three axes, 25 us, 4.0 TB/s.
 #include <stdint.h>
 
 #include "kb_internal.h"
@@ -33,6 +36,10 @@ struct RopeArgs {
 };
 
 constexpr int kBlock = 256;  // most threads of a block
+// Blocks per SM to aim for and the longest run of tokens per thread: fewer and
+// longer runs leave SMs idle at the end of large calls (64 tokens: 180 us instead
+// of 169 for 92,416), more and shorter ones convert frequencies too often (12
+// blocks: 29 us instead of 24 for 32,845 fp32 tokens).
 constexpr int kBlocksPerSm = 6, kMostTokens = 32;
 
 constexpr double kInvTwoPi = 0.15915494309189533576888;
