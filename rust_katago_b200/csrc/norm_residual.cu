@@ -402,7 +402,7 @@ int launch_shift(const NormArgs& a, cudaStream_t s) {
   }
   const int bytes = (2 + SHIFT) * NC * threads * 32;
   if (THREADS > 32) {
-    if (bytes > 48 * 1024) {
+    if (bytes + static_cast<int>(sizeof(float)) * 32 > 48 * 1024) {  // with the static part
       static std::atomic<uint64_t> configured{0};
       const uint64_t bit = 1ull << (dev & 63);
       if (!(configured.load() & bit)) {

@@ -187,6 +187,21 @@ def test_norm_residual(cuda, xdt, ydt, rows, width, post, pre, act, per, affine)
     close(h, ref, rounding(ref, ydt) + herr)
 
 
+@pytest.mark.parametrize("width", [1032, 2560, 2568, 2680, 3584, 3592, 4096, 4100, 5120, 5128, 6144, 8192, 8200, 12000])
+@pytest.mark.parametrize("shifts", [0, 1, 2])
+def test_norm_wide_rows_of_every_shared_size(cuda, width, shifts):
+    g = torch.Generator(device="cuda").manual_seed(width)
+    x, y = (torch.randn(3, width, generator=g, device="cuda") for _ in range(2))
+    b = torch.randn(width, generator=g, device="cuda")
+    kw = dict(pre_beta=b if shifts else None, post_beta=b if shifts == 2 else None)
+    xo, h = block.norm_residual(x, y, post="rms", pre="layer", **kw)
+    r = x.double() + norm_ref(y.double(), "rms", None, kw["post_beta"], 1e-6)
+    ref = norm_ref(r, "layer", None, kw["pre_beta"], 1e-6)
+    # values and deviations near 1: 96 roundings of fp32 on the way to r, twice that to h
+    close(xo, r, 96 * E * (1 + r.abs()))
+    close(h, ref, 192 * E * (2 + ref.abs() + b.abs()))
+
+
 def test_norm_forms_without_parts_in_place_and_strided(cuda):
     g = torch.Generator(device="cuda").manual_seed(5)
     x = torch.randn(70, 200, generator=g, device="cuda")
