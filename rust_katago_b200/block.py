@@ -94,6 +94,17 @@ def _check(t, what, shape, dtype, device):
     raise ValueError(f"{what}'s last dimension must be contiguous")
 
 
+def _status(t, device):
+    """The address of a status word [flags, first_layer] (None: 0)."""
+    if t is None:
+        return 0
+    if not isinstance(t, torch.Tensor) or t.dtype not in (torch.int32, torch.uint32):
+        raise TypeError("status must be an int32 or uint32 tensor")
+    if t.get_device() != device or t.dim() != 1 or t.shape[0] < 2 or not t.is_contiguous():
+        raise ValueError(f"status must be two contiguous elements on device {device}")
+    return t.data_ptr()
+
+
 @functools.cache
 def _native(name):
     """A function of the library (loaded at the first call), without the lookups of a call by name."""
@@ -251,6 +262,7 @@ def diff_attention(q, k, v, lam, *, gamma=None, out_scale=1.0, eps=1e-5, scale=N
     kv_lens[b] (int32 [batch]) and with key_mask[b, j] set (bool or uint8
     [batch, kv_len]); causal puts the queries at the end of the keys, window
     keeps the last `window` keys of each.  Queries that see no key give zeros.
+    status: a status word (int32 or uint32 [flags, first_layer], two elements).
     Returns out [batch, q_len, heads, 2 d].
     """
     device = _device(q, "q")
@@ -283,12 +295,13 @@ def diff_attention(q, k, v, lam, *, gamma=None, out_scale=1.0, eps=1e-5, scale=N
         _DTYPES[dtype], batch, q_len, kv_len, heads, kv_heads, d, bool(causal), window,
         d**-0.5 if scale is None else scale, out_scale, eps, qs[0], qs[1], qs[2], qs[3], ks[0], ks[1], ks[2], ks[3],
         vs[0], vs[1], vs[2], os[0], os[1], os[2], mask_batch)
+    sp = _status(status, device)
     need, wp = _workspace_bytes(desc, device), 0
     if need:
         work = _empty(q, need, torch.uint8, stream, device)
         wp = work.data_ptr()
     code = _native("kb_diff_attention")(desc, qp, kp, vp, lp, gp, np_, mp, op, wp, need,
-                                        0 if status is None else status.data_ptr(), _raw(stream, device))
+                                        sp, _raw(stream, device))
     if code:
         check(code)
     return out

@@ -509,3 +509,16 @@ def test_wrapper_refusals(cuda):
         block.norm_residual(x, x, gate=x[:3], rows_per_cond=2)
     with pytest.raises(ValueError):
         block.rope_axes(x.view(4, 3, 32), torch.zeros(1, 3, dtype=torch.int32, device="cuda"), torch.zeros(1, 16, 1, device="cuda"))
+
+
+def test_status_word_is_checked(cuda):
+    q, k, v, lam, _ = attn_inputs(1, 2, 8, 2, 2, 64, torch.bfloat16)
+    word = lambda *a, **kw: torch.zeros(*a, device="cuda", **{"dtype": torch.int32, **kw})  # noqa: E731
+    for status in (word(2, dtype=torch.float32), word(2, dtype=torch.int64), word(2, dtype=torch.int16), [0, 0], 5,
+                   word(2).cpu(), word(1), word(0), word(()), word(4)[::2], word(2, 2)):
+        with pytest.raises((TypeError, ValueError)):
+            block.diff_attention(q, k, v, lam, status=status)
+    ref = block.diff_attention(q, k, v, lam)
+    for status in (None, word(2), word(2, dtype=torch.uint32), word(6)[2:5]):
+        assert torch.equal(block.diff_attention(q, k, v, lam, status=status), ref)
+        assert status is None or status.cpu().view(torch.int32).tolist() == [0] * len(status)
