@@ -212,6 +212,9 @@ extern "C" int kb_diff_attention(const kb_diff_attention_desc* desc, const uint1
   for (const void* p : {static_cast<const void*>(q), static_cast<const void*>(k), static_cast<const void*>(v),
                         static_cast<const void*>(out), static_cast<const void*>(workspace)})
     if (reinterpret_cast<uintptr_t>(p) % 16) return bad("q, k, v, out and workspace must be 16-byte aligned");
+  for (const void* p : {static_cast<const void*>(lambda), static_cast<const void*>(gamma),
+                        static_cast<const void*>(kv_lens), static_cast<const void*>(status)})
+    if (reinterpret_cast<uintptr_t>(p) % 4) return bad("lambda, gamma, kv_lens and status must be 4-byte aligned");
   if (out == q || out == k || out == v) return bad("out must not be an input");
   size_t need = 0;
   kb_diff_attention_workspace(desc, &need);

@@ -618,6 +618,13 @@ extern "C" int kb_norm_residual(const kb_norm_residual_desc* desc, const void* x
     return bad("in place needs equal strides");
   if (h && (h == x || h == x_out)) return bad("h must not be x or x_out");
   if (x_out && x_out == y) return bad("x_out must not be y");
+  auto off = [](const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % (dtype == KB_DT_F32 ? 4 : 2) != 0; };
+  for (const void* p : {x, static_cast<const void*>(x_out)})
+    if (off(p, d.stream_dtype)) return bad("x and x_out must be aligned to their elements");
+  for (const void* p : {y, gate, mod_scale, mod_shift, static_cast<const void*>(h)})
+    if (off(p, d.branch_dtype)) return bad("y, gate, mod_scale, mod_shift and h must be aligned to their elements");
+  for (const float* p : {post_gamma, post_beta, pre_gamma, pre_beta})
+    if (off(p, KB_DT_F32)) return bad("gammas and betas must be aligned to their elements");
   NormArgs a{d, x, y, post_gamma, post_beta, pre_gamma, pre_beta, gate, mod_scale, mod_shift, x_out, h};
   if (a.d.rows_per_cond < 1) a.d.rows_per_cond = 1;
   // Eight columns per access need whole groups and 16-byte rows; type pairs that

@@ -281,6 +281,9 @@ extern "C" int kb_rope_axes(const void* x, int dtype, int tokens, int heads, int
   const int es = dtype == KB_DT_F32 ? 4 : 2;
   if (reinterpret_cast<uintptr_t>(x) % es || reinterpret_cast<uintptr_t>(out) % es)
     return bad("x and out must be aligned to their elements");
+  if (reinterpret_cast<uintptr_t>(positions) % 4 || reinterpret_cast<uintptr_t>(freqs) % 4 ||
+      reinterpret_cast<uintptr_t>(slots) % 8)
+    return bad("positions, freqs and slots must be aligned to their elements");
   // out's rows and heads must be disjoint, whichever of the two is outer
   const int64_t rows = slots ? out_rows : tokens, most = int64_t(1) << 40;
   if (x_token > most || x_head > most || out_token > most || out_head > most) return bad("strides above 2^40 elements");

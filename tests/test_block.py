@@ -130,3 +130,26 @@ def test_wrappers_refuse_cpu_tensors():
         block.norm_residual(x[0])
     with pytest.raises(TypeError):
         block.diff_attention(None, x, x, x)
+
+
+@pytest.mark.parametrize("kw", [dict(positions=P + 2), dict(freqs=P + 1), dict(slots=P + 4)])
+def test_rope_refuses_misaligned_tensors(kw):
+    invalid(rope(**kw))
+
+
+@pytest.mark.parametrize("ptr", [dict(x=P + 2), dict(y=P + 1), dict(pg=P + 2), dict(pb=P + 3), dict(qg=P + 1), dict(qb=P + 2),
+                                 dict(gate=P + 1), dict(ms=P + 1), dict(mt=P + 3), dict(x_out=3 * P + 2), dict(h=4 * P + 1)])
+def test_norm_refuses_misaligned_tensors(ptr):
+    invalid(norm(ptr))
+
+
+@pytest.mark.parametrize("ptr", [dict(lam=P + 2), dict(gamma=P + 1), dict(kv_lens=P + 2), dict(status=P + 2)])
+def test_attention_refuses_misaligned_tensors(ptr):
+    status = ptr.pop("status", 0)
+    if status:
+        d = 64
+        desc = _capi.DiffAttentionDesc(dtype=_capi.DT_BF16, batch=1, q_len=1, kv_len=1, heads=1, kv_heads=1, head_dim=d,
+                                       scale=1.0, out_scale=1.0, q_map=d, k_map=d)
+        invalid(_capi.load().kb_diff_attention(ctypes.byref(desc), P, P, P, P, 0, 0, 0, 2 * P, 0, 0, status, 0))
+    else:
+        invalid(attn(ptr))
