@@ -312,7 +312,8 @@ typedef struct kb_norm_residual_desc {
 /* y, gate, mod_scale, mod_shift, the gammas and the betas (fp32 [width]) may be
  * NULL (y: r = res_scale * x; gate: 1; mods: 0; gamma: 1; beta: 0); x_out or h
  * may be NULL when it is not wanted, not both.  x_out may be x, and h may be y,
- * with the same stride. */
+ * with the same stride; with rows_per_cond 1 h may also be the gate or a
+ * modulation of the same stride.  No other tensor may be an output. */
 KB_API int kb_norm_residual(const kb_norm_residual_desc* desc, const void* x, const void* y, const float* post_gamma,
                             const float* post_beta, const float* pre_gamma, const float* pre_beta, const void* gate,
                             const void* mod_scale, const void* mod_shift, void* x_out, void* h, uintptr_t stream);

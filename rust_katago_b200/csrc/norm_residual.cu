@@ -618,6 +618,13 @@ extern "C" int kb_norm_residual(const kb_norm_residual_desc* desc, const void* x
     return bad("in place needs equal strides");
   if (h && (h == x || h == x_out)) return bad("h must not be x or x_out");
   if (x_out && x_out == y) return bad("x_out must not be y");
+  // What rows share is read while other rows are written; a row of its own per
+  // row is read before h's.
+  for (const void* p : {static_cast<const void*>(post_gamma), static_cast<const void*>(post_beta),
+                        static_cast<const void*>(pre_gamma), static_cast<const void*>(pre_beta), gate, mod_scale, mod_shift})
+    if (p && (p == x_out || (p == h && (p == post_gamma || p == post_beta || p == pre_gamma || p == pre_beta ||
+                                        (d.rows > 1 && (d.rows_per_cond != 1 || d.cond_stride != d.h_stride))))))
+      return bad("x_out and h must not be a gamma, a beta, the gate or a modulation");
   auto off = [](const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % (dtype == KB_DT_F32 ? 4 : 2) != 0; };
   for (const void* p : {x, static_cast<const void*>(x_out)})
     if (off(p, d.stream_dtype)) return bad("x and x_out must be aligned to their elements");

@@ -153,3 +153,12 @@ def test_attention_refuses_misaligned_tensors(ptr):
         invalid(_capi.load().kb_diff_attention(ctypes.byref(desc), P, P, P, P, 0, 0, 0, 2 * P, 0, 0, status, 0))
     else:
         invalid(attn(ptr))
+
+
+@pytest.mark.parametrize("ptr,kw", [
+    (dict(gate=4 * P), dict(rows_per_cond=5)), (dict(ms=4 * P), dict(rows_per_cond=2)), (dict(mt=4 * P), dict(cond_stride=0)),
+    (dict(gate=4 * P), dict(cond_stride=192)), (dict(gate=3 * P), {}), (dict(ms=3 * P), dict(stream_dtype=_capi.DT_BF16)),
+    (dict(mt=3 * P), dict(rows_per_cond=5)), (dict(pg=4 * P), {}), (dict(pb=3 * P), {}), (dict(qg=3 * P), dict(rows=1)),
+    (dict(qb=4 * P), dict(rows=1))])
+def test_norm_refuses_outputs_over_what_rows_share(ptr, kw):
+    invalid(norm(ptr, **kw))

@@ -522,3 +522,18 @@ def test_status_word_is_checked(cuda):
     for status in (None, word(2), word(2, dtype=torch.uint32), word(6)[2:5]):
         assert torch.equal(block.diff_attention(q, k, v, lam, status=status), ref)
         assert status is None or status.cpu().view(torch.int32).tolist() == [0] * len(status)
+
+
+@pytest.mark.parametrize("width,ydt", [(256, torch.bfloat16), (1100, torch.float16), (9000, torch.bfloat16)])
+@pytest.mark.parametrize("name", ["gate", "mod_scale", "mod_shift"])
+def test_norm_output_in_place_of_a_condition_per_row(cuda, width, ydt, name):
+    g = torch.Generator(device="cuda").manual_seed(width)
+    x = torch.randn(700, width, generator=g, device="cuda")
+    y, gate, ms, mt = (torch.randn(700, width, generator=g, device="cuda").to(ydt) for _ in range(4))
+    cond = dict(gate=gate, mod_scale=ms, mod_shift=mt)
+    kw = dict(post="rms", pre="layer", rows_per_cond=1)
+    xo, h = block.norm_residual(x, y, **cond, **kw)
+    xi, hi = block.norm_residual(x, y, **cond, h=cond[name], **kw)
+    assert hi is cond[name] and torch.equal(xi, xo) and torch.equal(hi, h)
+    with pytest.raises(_capi.KbError):
+        block.norm_residual(x[:1], y[:1], pre="rms", pre_gamma=x[0], x_out=x[:1])
