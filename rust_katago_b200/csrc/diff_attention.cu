@@ -5,6 +5,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "kb_diff.cuh"
 #include "kb_internal.h"
 #include "kb_numeric.cuh"
@@ -162,9 +164,17 @@ int check_desc(const kb_diff_attention_desc* desc) {
     return bad("strides must be multiples of 8 elements, not negative and below 2^38");
   if ((d.q_len > 1 && d.q_token == 0) || (d.kv_len > 1 && (d.k_token == 0 || d.v_token == 0)))
     return bad("tokens cannot be broadcast");
-  auto apart = [&](int64_t stride, int64_t extent) { return extent <= 1 || stride >= 2 * d.head_dim; };
-  if (!apart(d.out_batch, d.batch) || !apart(d.out_token, d.q_len) || !apart(d.out_head, d.heads))
-    return bad("out's rows must not overlap");
+  // out's dimensions nest: each steps over all that the smaller ones span.
+  struct Dim {
+    int64_t stride, extent;
+  } dims[3] = {{d.out_batch, d.batch}, {d.out_token, d.q_len}, {d.out_head, d.heads}};
+  std::sort(dims, dims + 3, [](const Dim& x, const Dim& y) { return x.stride < y.stride; });
+  int64_t span = 2 * d.head_dim;
+  for (const Dim& m : dims) {
+    if (m.extent <= 1) continue;
+    if (m.stride < span) return bad("out's rows must not overlap");
+    span = m.stride > most / m.extent ? most : span + m.stride * (m.extent - 1);  // (no stride reaches `most`)
+  }
   if (d.mask_batch < 0 || d.mask_batch > most) return bad("mask_batch");
   return KB_OK;
 }

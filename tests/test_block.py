@@ -162,3 +162,23 @@ def test_attention_refuses_misaligned_tensors(ptr):
     (dict(qb=4 * P), dict(rows=1))])
 def test_norm_refuses_outputs_over_what_rows_share(ptr, kw):
     invalid(norm(ptr, **kw))
+
+
+@pytest.mark.parametrize("kw", [
+    dict(out_token=128, out_head=128), dict(out_batch=512, out_token=512), dict(out_batch=128, out_token=512, out_head=128),
+    dict(out_token=128, out_head=8 * 128 - 8), dict(out_batch=8 * 512 - 8), dict(out_batch=128, out_token=248, out_head=8 * 512)])
+def test_attention_refuses_outputs_that_overlap(kw):
+    invalid(attn(**kw))
+
+
+@pytest.mark.parametrize("kw", [
+    dict(out_token=128, out_head=8 * 128), dict(out_token=520, out_batch=7 * 520 + 512), dict(out_batch=136, out_token=272, out_head=8 * 272),
+    dict(out_batch=128, out_token=4 * 256, out_head=256), dict(q_len=1, out_token=0), dict(batch=1, out_batch=8)])
+def test_attention_takes_any_nested_output(kw):
+    """A descriptor that is right (asked for its workspace: no device needed)."""
+    need = ctypes.c_size_t()
+    d = dict(dtype=_capi.DT_BF16, batch=2, q_len=8, kv_len=16, heads=4, kv_heads=2, head_dim=64, causal=1, scale=0.125,
+             out_scale=1.0, eps=1e-5, q_batch=4096, q_token=512, q_head=128, q_map=64, k_batch=4096, k_token=256, k_head=128,
+             k_map=64, v_batch=4096, v_token=256, v_head=128, out_batch=4096, out_token=512, out_head=128)
+    desc = _capi.DiffAttentionDesc(**{**d, **kw})
+    assert _capi.load().kb_diff_attention_workspace(ctypes.byref(desc), ctypes.byref(need)) == _capi.KB_OK
