@@ -455,6 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1) diff_tc_kernel(const __grid_const
         release();
         continue;
       }
+      const bool seen = v0.y != 0.0f || v1.y != 0.0f;  // a row without keys is zero whatever eps and gamma are
       const float w0 = v0.y == 0.0f ? 0.0f : 1.0f / v0.y;
       const float w1 = v1.y == 0.0f ? 0.0f : lambda / v1.y;
       uint16_t* out = a.out + b * a.d.out_batch + i * a.d.out_token + h * a.d.out_head;
@@ -504,7 +505,8 @@ __global__ void __launch_bounds__(kThreads, 1) diff_tc_kernel(const __grid_const
         if (live) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            *reinterpret_cast<uint4*>(out + 32 * c + 8 * k) = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+            *reinterpret_cast<uint4*>(out + 32 * c + 8 * k) =
+                seen ? make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]) : make_uint4(0, 0, 0, 0);
         }
       }
     }

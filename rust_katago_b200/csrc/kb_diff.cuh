@@ -67,9 +67,11 @@ __device__ __forceinline__ int64_t row_index(const DiffArgs& a, int b, int i, in
 
 // A row's result from both maps' sums `acc` (kE dims per lane, dims lane kE..)
 // and weights `ll`: the weighted difference, its norm, one rounding.  Whole warps.
+// A row that saw no key is zero whatever eps and gamma are (0 / sqrt(0) is not).
 template <int kE>
 __device__ __forceinline__ void finish_row(const DiffArgs& a, int b, int i, int h, int lane, const float (&acc)[2][kE],
                                            const float (&ll)[2]) {
+  const bool seen = ll[0] != 0.0f || ll[1] != 0.0f;
   const float w0 = ll[0] == 0.0f ? 0.0f : 1.0f / ll[0];  // 0: no key was seen
   const float w1 = ll[1] == 0.0f ? 0.0f : a.lambda[h] / ll[1];
   float r[kE], ss = 0.0f;
@@ -89,7 +91,7 @@ __device__ __forceinline__ void finish_row(const DiffArgs& a, int b, int i, int 
 #pragma unroll
   for (int e = 0; e < kE; e += 2) {
     const float g0 = a.gamma ? a.gamma[lane * kE + e] : 1.0f, g1 = a.gamma ? a.gamma[lane * kE + e + 1] : 1.0f;
-    w[e / 2] = pack16x2(make_float2(r[e] * f * g0, r[e + 1] * f * g1), a.d.dtype == KB_DT_F16);
+    w[e / 2] = seen ? pack16x2(make_float2(r[e] * f * g0, r[e + 1] * f * g1), a.d.dtype == KB_DT_F16) : 0u;
   }
   if constexpr (kE == 4) *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
   else *reinterpret_cast<uint32_t*>(out) = w[0];

@@ -537,3 +537,29 @@ def test_norm_output_in_place_of_a_condition_per_row(cuda, width, ydt, name):
     assert hi is cond[name] and torch.equal(xi, xo) and torch.equal(hi, h)
     with pytest.raises(_capi.KbError):
         block.norm_residual(x[:1], y[:1], pre="rms", pre_gamma=x[0], x_out=x[:1])
+
+
+# batch, q_len, kv_len, heads, kv_heads, lens, mask: rows without keys through every end of both kernels (one block,
+# a cluster, parts in the workspace; tiles of 128 queries with and without keys)
+UNSEEN = [(2, 1, 40, 2, 2, [40, 0], None), (1, 3, 1000, 2, 2, [2], None), (2, 1, 60000, 1, 1, [60000, 0], None),
+          (2, 200, 200, 2, 2, None, "empty"), (2, 300, 300, 2, 2, [20, 0], None), (1, 160, 6000, 1, 1, [90], None)]
+
+
+@pytest.mark.parametrize("d,dtype", [(64, torch.bfloat16), (32, torch.float16)])
+@pytest.mark.parametrize("case", UNSEEN, ids=lambda c: "-".join(str(x) for x in c[:5]))
+def test_queries_without_keys_are_zero_for_any_eps_and_gamma(cuda, d, dtype, case):
+    batch, q_len, kv_len, heads, kv_heads, lens, mask = case
+    q, k, v, lam, gamma = attn_inputs(batch, q_len, kv_len, heads, kv_heads, d, dtype, seed=q_len)
+    kv_lens = None if lens is None else torch.tensor(lens, dtype=torch.int32, device="cuda")
+    key_mask = make_mask(mask, batch, kv_len)
+    see = visible(batch, q_len, kv_len, True, 0, kv_lens, key_mask)
+    hidden = ~see.any(-1)
+    assert hidden.any()
+    kw = dict(causal=True, kv_lens=kv_lens, key_mask=key_mask, eps=0.0)
+    got = block.diff_attention(q, k, v, lam, gamma=gamma, **kw)
+    ref, bound = attn_ref(q, k, v, lam, gamma, see, 1.0, 0.0, d**-0.5)
+    assert (got[hidden] == 0).all()
+    seen = ~hidden
+    close(got[seen], ref[seen], bound[seen])
+    gamma[3] = float("inf")
+    assert (block.diff_attention(q, k, v, lam, gamma=gamma, **kw)[hidden] == 0).all()
