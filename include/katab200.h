@@ -327,9 +327,11 @@ KB_API int kb_norm_residual(const kb_norm_residual_desc* desc, const void* x, co
  * heads, 2 * head_dim], all of dtype KB_DT_F16 or KB_DT_BF16.
  * Keys: those below kv_lens[b] (nullable, int32 [batch], clamped to [0,
  * kv_len]) whose key_mask byte (nullable, [batch, kv_len], row stride
- * mask_batch) is nonzero.  causal: query i of a sequence of n keys sits at
+ * mask_batch) is nonzero.  causal: query i of a sequence of n tokens sits at
  * position n - q_len + i and sees the keys up to there, with window > 0 only
- * the last `window` of them.  A query that sees no key gets zeros.  What lies
+ * those of the last `window` positions; n is kv_lens[b] (below 0: 0; without
+ * kv_lens kv_len) even above kv_len, where K and V hold the first kv_len of the
+ * sequence.  A query that sees no key gets zeros, whatever eps is.  What lies
  * in K and V at keys that kv_lens or key_mask hide is never used, NaN and
  * infinities included; a non-finite value of V at a key that only the causal
  * mask or the window hides may reach other queries of the call.

@@ -260,8 +260,9 @@ def diff_attention(q, k, v, lam, *, gamma=None, out_scale=1.0, eps=1e-5, scale=N
     kv_len, kv_heads, 2 d], d 32 or 64, bf16 or fp16; lam fp32 [heads]; gamma
     fp32 [2 d] or None (no norm); scale defaults to d ** -0.5.  Keys: below
     kv_lens[b] (int32 [batch]) and with key_mask[b, j] set (bool or uint8
-    [batch, kv_len]); causal puts the queries at the end of the keys, window
-    keeps the last `window` keys of each.  Queries that see no key give zeros.
+    [batch, kv_len]); causal puts the queries at the end of the sequence (of
+    kv_lens[b] tokens, of which k and v may hold only the first kv_len), window
+    keeps the last `window` positions of each.  Queries that see no key give zeros.
     status: a status word (int32 or uint32 [flags, first_layer], two elements).
     Returns out [batch, q_len, heads, 2 d].
     """

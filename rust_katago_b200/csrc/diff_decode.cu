@@ -126,16 +126,16 @@ __global__ void __launch_bounds__(32 * kWarps, 2) diff_decode_kernel(const DiffA
   const int rows = min(kRows, d.q_len * share - r0);  // valid rows of this tile
 
   // Keys of the tile, of this split, and of each row held by this thread.
-  const int n = key_count(a, b);
-  int first, last;
-  key_range_n(d, n, r0 / share, (r0 + rows - 1) / share, first, last);
+  int off, first, last;
+  const int n = key_count(a, b, off);
+  key_range_n(d, n, off, r0 / share, (r0 + rows - 1) / share, first, last);
   const int steps = (max(0, last - first) + 15) / 16;
   const int per = (steps + splits - 1) / splits * 16;
   const int s0 = min(last, first + split * per), s1 = min(last, s0 + per);
   int common_lo = 0, common_hi = n;  // keys that every row sees
   if (d.causal) {
-    common_hi = min(n, n - d.q_len + r0 / share + 1);
-    if (d.window) common_lo = max(0, n - d.q_len + (r0 + rows - 1) / share + 1 - d.window);
+    common_hi = min(n, off + r0 / share + 1);
+    if (d.window) common_lo = max(d.window, off + (r0 + rows - 1) / share + 1) - d.window;
   }
   int lo[NR][2], hi[NR][2];
 #pragma unroll
@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) diff_decode_kernel(const DiffA
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int r = r0 + 8 * t + 2 * c + u;
-      key_range_n(d, n, r / share, r / share, lo[t][u], hi[t][u]);
+      key_range_n(d, n, off, r / share, r / share, lo[t][u], hi[t][u]);
     }
   const uint8_t* mask = a.key_mask ? a.key_mask + b * d.mask_batch : nullptr;
 

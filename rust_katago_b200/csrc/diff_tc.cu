@@ -109,11 +109,11 @@ __device__ __forceinline__ void item_of(const DiffArgs& a, const Items& it, int 
 }
 
 // Key tiles [t0, t1) of an item.
-__device__ __forceinline__ void tiles_of(const DiffArgs& a, const Items& it, int b, int qt, int split, int& n, int& t0,
-                                         int& t1) {
-  n = key_count(a, b);
+__device__ __forceinline__ void tiles_of(const DiffArgs& a, const Items& it, int b, int qt, int split, int& n, int& off,
+                                         int& t0, int& t1) {
+  n = key_count(a, b, off);
   int first, last;
-  key_range_n(a.d, n, qt * kTile, min(a.d.q_len, qt * kTile + kTile) - 1, first, last);
+  key_range_n(a.d, n, off, qt * kTile, min(a.d.q_len, qt * kTile + kTile) - 1, first, last);
   const int lo = first / kTile, hi = last > first ? (last + kTile - 1) / kTile : lo;
   const int per = static_cast<int>(it.by_splits.div(hi - lo + it.splits - 1));
   t0 = min(hi, lo + split * per);
@@ -134,9 +134,9 @@ struct Walk {
   bool valid;
   __device__ __forceinline__ void seek(const DiffArgs& a, const Items& it) {
     for (int at; (at = item_at(round)) < it.count; ++round) {
-      int split, n, b, h, qt;
+      int split, n, off, b, h, qt;
       item_of(a, it, at, b, h, qt, split);
-      tiles_of(a, it, b, qt, split, n, t0, t1);
+      tiles_of(a, it, b, qt, split, n, off, t0, t1);
       if (t0 < t1) {
         t = t0;
         valid = true;
@@ -298,15 +298,15 @@ __global__ void __launch_bounds__(kThreads, 1) diff_tc_kernel(const __grid_const
     int tile = 0, busy = 0;  // tiles and items with keys so far
     bool ok = true;
     for (int round = 0, at; ok && (at = item_at(round)) < items.count; ++round) {
-      int b, h, qt, split, n, t0, t1;
+      int b, h, qt, split, n, off, t0, t1;
       item_of(a, items, at, b, h, qt, split);
-      tiles_of(a, items, b, qt, split, n, t0, t1);
+      tiles_of(a, items, b, qt, split, n, off, t0, t1);
       if (t0 >= t1) continue;
       int lo, hi, common_lo, common_hi, x0, x1;
       const int i0 = qt * kTile, i1 = min(a.d.q_len, i0 + kTile) - 1, i = min(i0 + row, i1);
-      key_range_n(a.d, n, i, i, lo, hi);
-      key_range_n(a.d, n, i1, i1, common_lo, x1);
-      key_range_n(a.d, n, i0, i0, x0, common_hi);
+      key_range_n(a.d, n, off, i, i, lo, hi);
+      key_range_n(a.d, n, off, i1, i1, common_lo, x1);
+      key_range_n(a.d, n, off, i0, i0, x0, common_hi);
       const int obuf = busy % G::kOBufs;
       const uint32_t o_addr = tmem + lanes + G::kO + (2 * obuf + map) * G::kDv;
       float m = -INFINITY, l = 0.0f;
@@ -410,9 +410,9 @@ __global__ void __launch_bounds__(kThreads, 1) diff_tc_kernel(const __grid_const
     const int row = threadIdx.x & (kTile - 1);
     int busy = 0;
     for (int round = 0, at; (at = item_at(round)) < items.count; ++round) {
-      int b, h, qt, split, n, t0, t1;
+      int b, h, qt, split, n, off, t0, t1;
       item_of(a, items, at, b, h, qt, split);
-      tiles_of(a, items, b, qt, split, n, t0, t1);
+      tiles_of(a, items, b, qt, split, n, off, t0, t1);
       const int i = qt * kTile + row, obuf = busy % G::kOBufs;
       const uint32_t o_addr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + G::kO + 2 * obuf * G::kDv;
       const bool live = i < a.d.q_len;
@@ -600,9 +600,9 @@ __global__ void __launch_bounds__(kThreads, 1) diff_tc_kernel(const __grid_const
         int tile = 0, tile_v = 0, busy = 0;  // K tiles, V tiles and items loaded
         bool ok = true;
         for (int round = 0, at; ok && (at = item_at(round)) < items.count; ++round) {
-          int b, h, qt, split, n, t0, t1;
+          int b, h, qt, split, n, off, t0, t1;
           item_of(a, items, at, b, h, qt, split);
-          tiles_of(a, items, b, qt, split, n, t0, t1);
+          tiles_of(a, items, b, qt, split, n, off, t0, t1);
           if (t0 >= t1) continue;
           const int hk = h / share, qb = busy & 1;
           ok = wait_short(&q_empty[qb], ((busy >> 1) & 1) ^ 1, abort_flag);
@@ -643,9 +643,9 @@ __global__ void __launch_bounds__(kThreads, 1) diff_tc_kernel(const __grid_const
       int tile = 0;
       bool ok = true;
       for (int round = 0, at; ok && (at = item_at(round)) < items.count; ++round) {
-        int b, h, qt, split, n, t0, t1;
+        int b, h, qt, split, n, off, t0, t1;
         item_of(a, items, at, b, h, qt, split);
-        tiles_of(a, items, b, qt, split, n, t0, t1);
+        tiles_of(a, items, b, qt, split, n, off, t0, t1);
         const uint8_t* mask = has_mask ? a.key_mask + b * a.d.mask_batch : nullptr;
         for (int t = t0; t < t1; ++t, ++tile) {
           const int stage = tile % kS;

@@ -31,7 +31,7 @@ inline DiffArgs make_diff_args(const kb_diff_attention_desc& desc, const uint16_
   DiffArgs a{desc, q, k, v, lambda, gamma, kv_lens, key_mask, out, desc.scale * 1.4426950408889634f,
              nullptr, nullptr};
   kb_diff_attention_desc& d = a.d;
-  if (d.window >= d.kv_len) d.window = 0;  // hides nothing (and would overflow positions)
+  if (!kv_lens && d.window >= d.kv_len) d.window = 0;  // hides nothing
   if (d.batch == 1) d.q_batch = d.k_batch = d.v_batch = d.out_batch = d.mask_batch = 0;
   if (d.q_len == 1) d.q_token = d.out_token = 0;
   if (d.kv_len <= 1) d.k_token = d.v_token = 0;
@@ -40,25 +40,26 @@ inline DiffArgs make_diff_args(const kb_diff_attention_desc& desc, const uint16_
   return a;
 }
 
-// Keys of sequence b, kv_lens clamped to what K and V hold.
-__device__ __forceinline__ int key_count(const DiffArgs& a, int b) {
-  return a.kv_lens ? max(0, min(a.kv_lens[b], a.d.kv_len)) : a.d.kv_len;
+// Keys of sequence b, kv_lens clamped to what K and V hold, and the position of
+// its query 0: kv_lens - q_len, negative when there are more queries than keys.
+// A sequence longer than K and V hold keeps its positions (up to where those of
+// a tile's unused rows would pass 31 bits).
+__device__ __forceinline__ int key_count(const DiffArgs& a, int b, int& off) {
+  const int n = a.kv_lens ? max(0, min(a.kv_lens[b], 0x7fffff00)) : a.d.kv_len;
+  off = n - a.d.q_len;
+  return min(n, a.d.kv_len);
 }
 
 // [first, last): the keys that some of the queries i0..i1 of a sequence of n
-// keys sees, before the key mask.
-__device__ __forceinline__ void key_range_n(const kb_diff_attention_desc& d, int n, int i0, int i1, int& first,
+// keys sees, before the key mask.  first may lie past the last key.
+__device__ __forceinline__ void key_range_n(const kb_diff_attention_desc& d, int n, int off, int i0, int i1, int& first,
                                             int& last) {
   first = 0;
   last = n;
   if (d.causal) {
-    const int off = n - d.q_len;  // position of query 0, negative when there are more queries than keys
     last = max(0, min(n, off + i1 + 1));
-    if (d.window) first = max(0, off + i0 + 1 - d.window);
+    if (d.window) first = max(d.window, off + i0 + 1) - d.window;
   }
-}
-__device__ __forceinline__ void key_range(const DiffArgs& a, int b, int i0, int i1, int& first, int& last) {
-  key_range_n(a.d, key_count(a, b), i0, i1, first, last);
 }
 
 __device__ __forceinline__ int64_t row_index(const DiffArgs& a, int b, int i, int h) {

@@ -26,7 +26,11 @@ BOARD = 19
 
 
 class Cache:
-    """Rotated keys and the values of `batch` sequences, `capacity` tokens each: one row per token, [K | V]."""
+    """Rotated keys and the values of `batch` sequences, `capacity` tokens each: one row per token, [K | V].
+
+    lens counts the tokens that every sequence has had.  Those past the capacity get no row: they see the tokens
+    that have one and are seen by none.
+    """
 
     def __init__(self, batch: int, capacity: int, kv_heads: int, head_dim: int):
         self.batch, self.capacity = batch, capacity

@@ -563,3 +563,21 @@ def test_queries_without_keys_are_zero_for_any_eps_and_gamma(cuda, d, dtype, cas
     close(got[seen], ref[seen], bound[seen])
     gamma[3] = float("inf")
     assert (block.diff_attention(q, k, v, lam, gamma=gamma, **kw)[hidden] == 0).all()
+
+
+@pytest.mark.parametrize("d,dtype", [(64, torch.bfloat16), (32, torch.float16)])
+@pytest.mark.parametrize("q_len,kv_len,lens,window", [
+    (6, 4, [6, 4, 0], 0), (1, 300, [300, 301, 2**31 - 1], 0), (5, 1000, [1003, 1200, 40], 30), (1, 900, [930, 1500, 900], 700),
+    (200, 150, [200, 230, 90], 0), (300, 400, [460, 700, 900], 350), (140, 5000, [5100, 9000, 77], 5000)])
+def test_positions_of_sequences_longer_than_their_keys(cuda, d, dtype, q_len, kv_len, lens, window):
+    q, k, v, lam, gamma = attn_inputs(3, q_len, kv_len, 2, 1, d, dtype, seed=q_len)
+    kv_lens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    at = torch.arange(kv_len, device="cuda")
+    pos = kv_lens.long()[:, None, None] - q_len + torch.arange(q_len, device="cuda")[:, None]
+    see = (at <= pos) & (at < kv_lens[:, None, None])
+    if window:
+        see &= at > pos - window
+    got = block.diff_attention(q, k, v, lam, gamma=gamma, eps=1e-4, causal=True, window=window, kv_lens=kv_lens)
+    ref, bound = attn_ref(q, k, v, lam, gamma, see, 1.0, float(torch.tensor(1e-4)), d**-0.5)
+    close(got, ref, bound)
+    assert (got[~see.any(-1)] == 0).all()

@@ -88,3 +88,23 @@ def test_full_cache_drops_further_tokens(cuda):
     x = torch.randn(1, 6, 384, device="cuda").bfloat16()
     out, _ = net(x, torch.zeros(3, 6, dtype=torch.int32, device="cuda"), cache)
     assert torch.isfinite(out).all() and cache.slots(1).tolist() == [-1]
+
+
+def test_tokens_that_do_not_fit_leave_the_others_right(cuda):
+    width, d, capacity, n = 384, 32, 5, 9
+    net = diff_block.DiffBlock.random(width, 6, 6, d, seed=8)
+    x = torch.randn(2, n, width, generator=torch.Generator("cuda").manual_seed(3), device="cuda").bfloat16()
+    pos = diff_block.board_positions(1, 1)[:, :n].repeat(1, 2).contiguous()
+    at = torch.arange(n, device="cuda")
+    ref, _ = reference(net, x, pos, (at <= at[:, None]) & (at < capacity))  # tokens past the capacity see all that fitted
+    for pieces in ((9,), (3, 4, 1, 1), (5, 1, 3)):
+        cache = diff_block.Cache(2, capacity, 6, d)
+        outs, first = [], 0
+        for new in pieces:
+            p = pos.view(3, 2, n)[:, :, first : first + new].reshape(3, -1).contiguous()
+            outs.append(net(x[:, first : first + new].contiguous(), p, cache)[0])
+            first += new
+        got = torch.cat(outs, 1)
+        for i in range(n):
+            assert off(got[:, i], ref[:, i]) <= BOUND, (pieces, i)
+        assert cache.lens.tolist() == [n, n]
