@@ -274,6 +274,7 @@ KB_API int kb_attention_amax(const uint16_t* qkv, uint16_t* out, uint32_t* row_a
  * table with one nonzero axis per pair gives the sectioned form (time, height,
  * width); two axes with learned frequencies are the trunk's.  The angle is
  * summed and reduced to one turn in 64 bits, so long positions cost no accuracy.
+ * Pairs with a NaN or an infinity among their frequencies become NaN.
  * slots (nullable, int64 [tokens]): token t goes to row slots[t] of out instead
  * of row t; rows outside [0, out_rows) are not written (out_rows is ignored
  * without slots).  out may be x with the same strides and no slots; any other

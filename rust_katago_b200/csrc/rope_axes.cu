@@ -16,6 +16,7 @@
 // Measured: that case 162 us, 5.25 TB/s (0.80 of the copy rate), bound by the
 // bytes that 480 threads of 128 registers keep in flight; 32,845 tokens of 12 x 32
 // fp32, three axes, 25 us, 4.0 TB/s.
+#include <math.h>
 #include <stdint.h>
 
 #include "kb_internal.h"
@@ -115,11 +116,48 @@ __device__ __forceinline__ uint4 load(const uint4* p) {
 __device__ __forceinline__ uint16_t load(const uint16_t* p) { return *p; }
 __device__ __forceinline__ float load(const float* p) { return *p; }
 
+// An item with a NaN or an infinity among its frequencies, which no fixed-point
+// angle is: element by element, the pairs of such a frequency become NaN.  A
+// function of its own, entered before the frequencies are converted: inside the
+// loop over tokens it cost up to 33 registers (128 to 161 with 3 axes in pairs).
+template <typename T, int VE, bool HALVES, int AXES>
+__device__ __noinline__ void rotate_broken_item(const RopeArgs& a, const T* src, T* dst, const float* f, int o0, int o1,
+                                                int rotated, int64_t t0, int64_t end) {
+  const bool f16 = a.f16;
+  for (int64_t t = t0; t < end; t += a.block_tokens) {
+    const int64_t row = a.slots ? a.slots[t] : t;
+    if (row < 0 || (a.slots && row >= a.out_rows)) continue;
+    for (int p = 0; p < VE; ++p) {
+      const int at[2] = {HALVES ? o0 + p : o0 + 2 * p, HALVES ? o1 + p : o0 + 2 * p + 1};
+      T e[2] = {src[t * a.x_token + at[0]], src[t * a.x_token + at[1]]};
+      if (p < rotated) {
+        uint32_t angle = 0;
+        bool broken = false;
+        for (int x = 0; x < AXES; ++x) {
+          const int pos = a.positions[static_cast<int64_t>(x) * a.tokens + t];
+          const Turns freq = turns_of(f[p * AXES + x]);
+          broken = broken || !(fabsf(f[p * AXES + x]) < INFINITY);
+          angle += static_cast<uint32_t>(pos) * static_cast<uint32_t>(freq.high) + static_cast<uint32_t>(__mulhi(pos, freq.low));
+        }
+        float u, v;
+        if constexpr (sizeof(T) == 2) u = from16(e[0], f16), v = from16(e[1], f16);
+        else u = e[0], v = e[1];
+        float cs, sn;
+        cos_sin<sizeof(T) == 4>(static_cast<int32_t>(angle), cs, sn);
+        const float r = broken ? NAN : u * cs - v * sn, i = broken ? NAN : u * sn + v * cs;
+        if constexpr (sizeof(T) == 2) e[0] = bits16(r, f16), e[1] = bits16(i, f16);
+        else e[0] = r, e[1] = i;
+      }
+      dst[row * a.out_token + at[0]] = e[0], dst[row * a.out_token + at[1]] = e[1];
+    }
+  }
+}
+
 // A thread's item: 2 VE elements of one head, VE of them at o0 and VE at o1.
 // KB_ROPE_HALVES: u at o0 and v at o1 for pairs o0..; KB_ROPE_PAIRS: the pairs
 // o0/2.. lie interleaved across both.  VE = 1 takes any alignment.
 template <typename T, int VE, bool HALVES, int AXES>
-__global__ void __launch_bounds__(kBlock) rope_axes_kernel(const RopeArgs a) {
+__global__ void __launch_bounds__(kBlock) rope_axes_kernel(const __grid_constant__ RopeArgs a) {
   constexpr int kUnroll = 2;
   using R = typename Raw<T, VE>::type;
   // The block's threads: its items of one token, then of the next.
@@ -140,20 +178,29 @@ __global__ void __launch_bounds__(kBlock) rope_axes_kernel(const RopeArgs a) {
       rotated = max(0, min(VE, a.pairs - c * VE));
     }
   }
-  Turns freq[VE][AXES];
-  if (rotated) {
-    const float* f = a.freqs + static_cast<int64_t>(head) * a.freq_head_stride + c * VE * AXES;
-#pragma unroll
-    for (int p = 0; p < VE; ++p)
-#pragma unroll
-      for (int x = 0; x < AXES; ++x) freq[p][x] = p < rotated ? turns_of(f[p * AXES + x]) : Turns{0, 0};
-  }
   const T* src = static_cast<const T*>(a.x) + head * a.x_head;
   T* dst = static_cast<T*>(a.out) + head * a.out_head;
   const int step = a.block_tokens;
   const int64_t run = static_cast<int64_t>(step) * a.tokens_per_thread;
   int64_t t0 = blockIdx.y * run + sub;
   const int64_t end = min(static_cast<int64_t>(a.tokens), blockIdx.y * run + run);
+  Turns freq[VE][AXES];
+  if (rotated) {
+    const float* f = a.freqs + static_cast<int64_t>(head) * a.freq_head_stride + c * VE * AXES;
+    bool broken = false;
+#pragma unroll
+    for (int p = 0; p < VE; ++p)
+#pragma unroll
+      for (int x = 0; x < AXES; ++x) broken = broken || (p < rotated && !(fabsf(f[p * AXES + x]) < INFINITY));
+    if (broken) {
+      rotate_broken_item<T, VE, HALVES, AXES>(a, src, dst, f, o0, o1, rotated, t0, end);
+      return;
+    }
+#pragma unroll
+    for (int p = 0; p < VE; ++p)
+#pragma unroll
+      for (int x = 0; x < AXES; ++x) freq[p][x] = p < rotated ? turns_of(f[p * AXES + x]) : Turns{0, 0};
+  }
   // kUnroll tokens at a time, the next ones loaded before these are at work.
   R lo[kUnroll], hi[kUnroll];
   int pos[kUnroll][AXES];

@@ -581,3 +581,24 @@ def test_positions_of_sequences_longer_than_their_keys(cuda, d, dtype, q_len, kv
     ref, bound = attn_ref(q, k, v, lam, gamma, see, 1.0, float(torch.tensor(1e-4)), d**-0.5)
     close(got, ref, bound)
     assert (got[~see.any(-1)] == 0).all()
+
+
+@pytest.mark.parametrize("dtype,head_dim", [(torch.bfloat16, 64), (torch.float32, 64), (torch.float16, 20)])
+@pytest.mark.parametrize("layout", ["pairs", "halves"])
+@pytest.mark.parametrize("shared", [True, False])
+def test_rope_shows_non_finite_frequencies(cuda, dtype, head_dim, layout, shared):
+    pairs = head_dim // 2 - 2 if head_dim == 20 else head_dim // 4
+    x, pos, freqs = rope_inputs(300, 5, head_dim, pairs, 2, 1 if shared else 3, dtype, 100, seed=6)
+    clean = block.rope_axes(x, pos, freqs, rotary_heads=3, layout=layout)
+    freqs[0, 1, 0], freqs[0, 4, 1], freqs[-1, 7, 0] = float("nan"), float("inf"), -float("inf")
+    bad = torch.zeros(5, head_dim, dtype=torch.bool, device="cuda")
+    for h, p in ((0, 1), (0, 4), (2, 7)) if not shared else [(h, p) for h in range(3) for p in (1, 4, 7)]:
+        bad[h, [2 * p, 2 * p + 1] if layout == "pairs" else [p, p + pairs]] = True
+    for out in (None, x):  # x last: in place
+        got = block.rope_axes(x, pos, freqs, out, rotary_heads=3, layout=layout)
+        assert torch.isnan(got[:, bad]).all() and torch.equal(got[:, ~bad], clean[:, ~bad])
+    # a cache row that is skipped stays as it is
+    y, pos, _ = rope_inputs(4, 5, head_dim, pairs, 2, 1, dtype, 100, seed=7)
+    cache = torch.full((4, 5, head_dim), 3.0, dtype=dtype, device="cuda")
+    block.rope_axes(y, pos, freqs, cache, rotary_heads=3, layout=layout, slots=torch.tensor([2, -1, 9, 0], device="cuda"))
+    assert (cache[[1, 3]] == 3).all() and torch.isnan(cache[[0, 2]][:, bad]).all() and not torch.isnan(cache[:, ~bad]).any()
