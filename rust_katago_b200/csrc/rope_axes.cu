@@ -116,92 +116,90 @@ __device__ __forceinline__ uint4 load(const uint4* p) {
 __device__ __forceinline__ uint16_t load(const uint16_t* p) { return *p; }
 __device__ __forceinline__ float load(const float* p) { return *p; }
 
-// An item with a NaN or an infinity among its frequencies, which no fixed-point
-// angle is: element by element, the pairs of such a frequency become NaN.  A
-// function of its own, entered before the frequencies are converted: inside the
-// loop over tokens it cost up to 33 registers (128 to 161 with 3 axes in pairs).
+// Threads to compile for, which bounds the registers: 128 or 168 for the 16-byte
+// kernels of 16-bit types with 3 or 4 axes (both words of 24 or 32 frequencies
+// and the data of four tokens) and 64 for single elements with 3.  Left alone
+// they take up to 216, 168 and 66, and an SM holds a block less (90,000 tokens of
+// 36 x 64, halves: 192 instead of 179 us with 3 axes, 370 instead of 249 with 4;
+// 30,000 tokens of 30 pairs in halves, 3 axes: 157 instead of 144).
 template <typename T, int VE, bool HALVES, int AXES>
-__device__ __noinline__ void rotate_broken_item(const RopeArgs& a, const T* src, T* dst, const float* f, int o0, int o1,
-                                                int rotated, int64_t t0, int64_t end) {
-  const bool f16 = a.f16;
-  for (int64_t t = t0; t < end; t += a.block_tokens) {
-    const int64_t row = a.slots ? a.slots[t] : t;
-    if (row < 0 || (a.slots && row >= a.out_rows)) continue;
-    for (int p = 0; p < VE; ++p) {
-      const int at[2] = {HALVES ? o0 + p : o0 + 2 * p, HALVES ? o1 + p : o0 + 2 * p + 1};
-      T e[2] = {src[t * a.x_token + at[0]], src[t * a.x_token + at[1]]};
-      if (p < rotated) {
-        uint32_t angle = 0;
-        bool broken = false;
-        for (int x = 0; x < AXES; ++x) {
-          const int pos = a.positions[static_cast<int64_t>(x) * a.tokens + t];
-          const Turns freq = turns_of(f[p * AXES + x]);
-          broken = broken || !(fabsf(f[p * AXES + x]) < INFINITY);
-          angle += static_cast<uint32_t>(pos) * static_cast<uint32_t>(freq.high) + static_cast<uint32_t>(__mulhi(pos, freq.low));
-        }
-        float u, v;
-        if constexpr (sizeof(T) == 2) u = from16(e[0], f16), v = from16(e[1], f16);
-        else u = e[0], v = e[1];
-        float cs, sn;
-        cos_sin<sizeof(T) == 4>(static_cast<int32_t>(angle), cs, sn);
-        const float r = broken ? NAN : u * cs - v * sn, i = broken ? NAN : u * sn + v * cs;
-        if constexpr (sizeof(T) == 2) e[0] = bits16(r, f16), e[1] = bits16(i, f16);
-        else e[0] = r, e[1] = i;
-      }
-      dst[row * a.out_token + at[0]] = e[0], dst[row * a.out_token + at[1]] = e[1];
-    }
-  }
+constexpr int most_threads() {
+  if (VE == 1) return AXES == 3 ? 1024 : kBlock;
+  return sizeof(T) == 4 || AXES < 3 ? kBlock : AXES == 3 ? 512 : 384;
 }
 
 // A thread's item: 2 VE elements of one head, VE of them at o0 and VE at o1.
 // KB_ROPE_HALVES: u at o0 and v at o1 for pairs o0..; KB_ROPE_PAIRS: the pairs
 // o0/2.. lie interleaved across both.  VE = 1 takes any alignment.
-template <typename T, int VE, bool HALVES, int AXES>
-__global__ void __launch_bounds__(kBlock) rope_axes_kernel(const __grid_constant__ RopeArgs a) {
-  constexpr int kUnroll = 2;
-  using R = typename Raw<T, VE>::type;
-  // The block's threads: its items of one token, then of the next.
-  const int sub = threadIdx.x / a.block_items;
-  const int item = blockIdx.x * a.block_items + threadIdx.x - sub * a.block_items;
-  if (sub >= a.block_tokens || item >= a.items) return;
-  const int head = item / a.per_head, c = item - head * a.per_head;
-  const bool f16 = a.f16;
-  int o0 = 2 * VE * c, o1 = o0 + VE, rotated = 0;  // rotated: pairs of this item that turn
-  if (head < a.rotary_heads) {
-    if constexpr (HALVES) {
-      if (c * VE < a.pairs) {
-        o0 = c * VE;
-        o1 = a.pairs + o0;
-        rotated = VE;
+template <int VE, bool HALVES>
+struct Item {
+  int sub, head, c, o0, o1, rotated;  // sub: which of the block's tokens; rotated: pairs of this item that turn
+  // The block's threads: its items of one token, then of the next.  False for those left over.
+  __device__ __forceinline__ bool find(const RopeArgs& a) {
+    sub = threadIdx.x / a.block_items;
+    const int item = blockIdx.x * a.block_items + threadIdx.x - sub * a.block_items;
+    if (sub >= a.block_tokens || item >= a.items) return false;
+    head = item / a.per_head, c = item - head * a.per_head;
+    o0 = 2 * VE * c, o1 = o0 + VE, rotated = 0;
+    if (head < a.rotary_heads) {
+      if constexpr (HALVES) {
+        if (c * VE < a.pairs) {
+          o0 = c * VE;
+          o1 = a.pairs + o0;
+          rotated = VE;
+        }
+      } else {
+        rotated = max(0, min(VE, a.pairs - c * VE));
       }
-    } else {
-      rotated = max(0, min(VE, a.pairs - c * VE));
+    }
+    return true;
+  }
+};
+
+// The pairs of this thread's item that have a NaN or an infinity among their
+// frequencies become NaN: no fixed-point angle stands for those.  A function of
+// its own, after the loop over tokens and from nothing but the arguments, so that
+// the loop carries one register for it (a check in the loop took up to 41 more).
+template <typename T, int VE, bool HALVES, int AXES>
+__device__ __noinline__ void break_pairs(const RopeArgs& a) {
+  Item<VE, HALVES> it;
+  if (!it.find(a)) return;
+  const float* f = a.freqs + static_cast<int64_t>(it.head) * a.freq_head_stride + it.c * VE * AXES;
+  T* dst = static_cast<T*>(a.out) + it.head * a.out_head;
+  const int64_t run = static_cast<int64_t>(a.block_tokens) * a.tokens_per_thread;
+  const int64_t end = min(static_cast<int64_t>(a.tokens), blockIdx.y * run + run);
+  T nan;
+  if constexpr (sizeof(T) == 2) nan = bits16(NAN, a.f16);
+  else nan = NAN;
+  for (int p = 0; p < it.rotated; ++p) {
+    bool broken = false;
+    for (int x = 0; x < AXES; ++x) broken |= !(fabsf(f[p * AXES + x]) < INFINITY);
+    if (!broken) continue;
+    for (int64_t t = blockIdx.y * run + it.sub; t < end; t += a.block_tokens) {
+      const int64_t row = a.slots ? a.slots[t] : t;
+      if (row < 0 || (a.slots && row >= a.out_rows)) continue;
+      T* at = dst + row * a.out_token + it.o0 + (HALVES ? p : 2 * p);
+      at[0] = nan, at[HALVES ? it.o1 - it.o0 : 1] = nan;
     }
   }
+}
+
+template <typename T, int VE, bool HALVES, int AXES>
+__global__ void __launch_bounds__(most_threads<T, VE, HALVES, AXES>()) rope_axes_kernel(const __grid_constant__ RopeArgs a) {
+  constexpr int kUnroll = 2;
+  using R = typename Raw<T, VE>::type;
+  Item<VE, HALVES> it;
+  if (!it.find(a)) return;
+  const int head = it.head, o0 = it.o0, o1 = it.o1, rotated = it.rotated;
+  const bool f16 = a.f16;
   const T* src = static_cast<const T*>(a.x) + head * a.x_head;
   T* dst = static_cast<T*>(a.out) + head * a.out_head;
   const int step = a.block_tokens;
   const int64_t run = static_cast<int64_t>(step) * a.tokens_per_thread;
-  int64_t t0 = blockIdx.y * run + sub;
+  int64_t t0 = blockIdx.y * run + it.sub;
   const int64_t end = min(static_cast<int64_t>(a.tokens), blockIdx.y * run + run);
-  Turns freq[VE][AXES];
-  if (rotated) {
-    const float* f = a.freqs + static_cast<int64_t>(head) * a.freq_head_stride + c * VE * AXES;
-    bool broken = false;
-#pragma unroll
-    for (int p = 0; p < VE; ++p)
-#pragma unroll
-      for (int x = 0; x < AXES; ++x) broken = broken || (p < rotated && !(fabsf(f[p * AXES + x]) < INFINITY));
-    if (broken) {
-      rotate_broken_item<T, VE, HALVES, AXES>(a, src, dst, f, o0, o1, rotated, t0, end);
-      return;
-    }
-#pragma unroll
-    for (int p = 0; p < VE; ++p)
-#pragma unroll
-      for (int x = 0; x < AXES; ++x) freq[p][x] = p < rotated ? turns_of(f[p * AXES + x]) : Turns{0, 0};
-  }
-  // kUnroll tokens at a time, the next ones loaded before these are at work.
+  // kUnroll tokens at a time, the next ones loaded before these are at work (the
+  // first before the frequencies are converted).
   R lo[kUnroll], hi[kUnroll];
   int pos[kUnroll][AXES];
   int64_t row[kUnroll];
@@ -224,6 +222,22 @@ __global__ void __launch_bounds__(kBlock) rope_axes_kernel(const __grid_constant
     }
   };
   fetch(t0);
+  Turns freq[VE][AXES];
+  uint32_t worst = 0;  // the frequencies' largest magnitude, as bits
+  if (rotated) {
+    const float* f = a.freqs + static_cast<int64_t>(head) * a.freq_head_stride + it.c * VE * AXES;
+#pragma unroll
+    for (int p = 0; p < VE; ++p)
+#pragma unroll
+      for (int x = 0; x < AXES; ++x) {
+        freq[p][x] = Turns{0, 0};
+        if (p < rotated) {
+          const float v = f[p * AXES + x];
+          freq[p][x] = turns_of(v);
+          worst = max(worst, __float_as_uint(v) << 1);
+        }
+      }
+  }
   for (; t0 < end; t0 += kUnroll * step) {
     R now_lo[kUnroll], now_hi[kUnroll];
     int now_pos[kUnroll][AXES];
@@ -267,6 +281,7 @@ __global__ void __launch_bounds__(kBlock) rope_axes_kernel(const __grid_constant
       *reinterpret_cast<R*>(dst + now_row[u] * a.out_token + o1) = w1;
     }
   }
+  if (worst >= 0xff000000u) break_pairs<T, VE, HALVES, AXES>(a);
 }
 
 template <typename T, int VE, bool HALVES>
