@@ -87,6 +87,8 @@ class DiffBlock:
         board); causal lets a token see only itself and what came before."""
         batch, new, width = x.shape
         rows, d = batch * new, self.head_dim
+        if rows == 0:
+            return x.clone(), x.clone()
         flat = x.reshape(rows, width)
         _, h = block.norm_residual(flat, pre="rms", pre_gamma=self.pre_gamma, eps=self.eps, x_out=False)
         qkv = self._linear(h, self.wqkv)

@@ -108,3 +108,12 @@ def test_tokens_that_do_not_fit_leave_the_others_right(cuda):
         for i in range(n):
             assert off(got[:, i], ref[:, i]) <= BOUND, (pieces, i)
         assert cache.lens.tolist() == [n, n]
+
+
+@pytest.mark.parametrize("batch,new", [(2, 0), (0, 3), (0, 0)])
+def test_calls_without_tokens_do_nothing(cuda, batch, new):
+    net = diff_block.DiffBlock.random(384, 6, 2, 32, seed=9)
+    cache = diff_block.Cache(batch, 8, 2, 32)
+    x = torch.zeros(batch, new, 384, dtype=torch.bfloat16, device="cuda")
+    out, h = net(x, torch.zeros(3, batch * new, dtype=torch.int32, device="cuda"), cache)
+    assert out.shape == h.shape == (batch, new, 384) and cache.lens.tolist() == [0] * batch
