@@ -24,6 +24,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import functools
+import operator
 import struct
 
 import numpy as np
@@ -56,7 +57,13 @@ def _raw(stream, device):
     """The cudaStream_t of `stream` (None: the current stream) as an integer."""
     if stream is None:
         return _current_stream(device)
-    return stream if isinstance(stream, int) else stream.cuda_stream
+    return stream if isinstance(stream, int) else _cuda_stream(stream).cuda_stream
+
+
+def _cuda_stream(stream):
+    if not isinstance(stream, torch.cuda.Stream):
+        raise TypeError(f"stream must be a torch.cuda.Stream or a cudaStream_t as an integer, got {stream!r}")
+    return stream
 
 
 def _lookup(table, key, what):
@@ -68,9 +75,7 @@ def _lookup(table, key, what):
 
 def _device(t, what):
     """The device index of a CUDA tensor on the current device."""
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{what} must be a tensor")
-    index = t.get_device()
+    index = _tensor(t, what).get_device()
     if index < 0:
         raise ValueError(f"{what} must be a CUDA tensor")
     if index != _current_device():
@@ -78,13 +83,26 @@ def _device(t, what):
     return index
 
 
+def _tensor(t, what):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{what} must be a tensor")
+    return t
+
+
+def _pack(form, *values):
+    """A descriptor as bytes."""
+    try:
+        return form.pack(*values)
+    except struct.error as e:
+        raise ValueError(f"an argument is no 32-bit integer or no number: {e}") from None
+
+
 def _check(t, what, shape, dtype, device):
     """The address of `t`; raises unless it has this shape, type and device and a contiguous last dimension."""
     if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == device
             and (t.stride(-1) == 1 or shape[-1] < 2)):
         return t.data_ptr()
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{what} must be a tensor")
+    _tensor(t, what)
     if t.dtype is not dtype:
         raise TypeError(f"{what} must be {dtype}, got {t.dtype}")
     if t.get_device() != device:
@@ -115,7 +133,8 @@ def _on(stream, device):
     """The context in which tensors are allocated for a call on `stream`."""
     if stream is None:
         return contextlib.nullcontext()
-    return torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream)
+    return torch.cuda.stream(
+        torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else _cuda_stream(stream))
 
 
 def _empty(like, shape, dtype, stream, device):
@@ -137,11 +156,18 @@ def rope_axes(x, positions, freqs, out=None, *, rotary_heads=None, layout="pairs
     device = _device(x, "x")
     dtype, shape = x.dtype, x.shape
     kind = _lookup(_DTYPES, dtype, "x's dtype")
-    if len(shape) != 3 or freqs.dim() != 3:
+    if len(shape) != 3 or _tensor(freqs, "freqs").dim() != 3:
         raise ValueError("x must be [tokens, heads, head_dim] and freqs [heads, pairs, axes]")
     tokens, heads, head_dim = shape
     freq_shape = freqs.shape
     freq_heads, pairs, axes = freq_shape
+    rotary = heads
+    if rotary_heads is not None:
+        rotary = operator.index(rotary_heads)
+        if rotary < 0 or rotary > heads:
+            raise ValueError(f"rotary_heads must be 0..{heads}, got {rotary}")
+    if (tokens | heads | head_dim | freq_heads | pairs | axes) >> 31:
+        raise ValueError("no dimension may pass 2^31 - 1")
     xp = _check(x, "x", shape, dtype, device)
     pp = _check(positions, "positions", (axes, tokens), torch.int32, device)
     fp = _check(freqs, "freqs", freq_shape, torch.float32, device)
@@ -154,14 +180,14 @@ def rope_axes(x, positions, freqs, out=None, *, rotary_heads=None, layout="pairs
         out = _empty(x, shape, dtype, stream, device)
         op = out.data_ptr()
     else:
-        rows = out.shape[0]
+        rows = out.shape[0] if _tensor(out, "out").dim() else 0
         op = _check(out, "out", shape if slots is None else (rows, heads, head_dim), dtype, device)
         if slots is not None:
             sp = _check(slots, "slots", (tokens,), torch.int64, device)
     xs, os = x.stride(), out.stride()
     code = _native("kb_rope_axes")(
         xp, kind, tokens, heads, head_dim, xs[0], xs[1], pp, axes, fp, freq_heads, pairs,
-        heads if rotary_heads is None else rotary_heads, _lookup(_LAYOUTS, layout, "layout"), sp, rows, op, os[0],
+        rotary, _lookup(_LAYOUTS, layout, "layout"), sp, rows, op, os[0],
         os[1], _raw(stream, device))
     if code:
         check(code)
@@ -191,9 +217,9 @@ def norm_residual(x, y=None, *, post=None, pre=None, post_gamma=None, post_beta=
     xp = _check(x, "x", shape, dtype, device)
     yp = y_stride = 0
     if y is not None:
-        if h_dtype is not None and h_dtype != y.dtype:
+        if h_dtype is not None and h_dtype != _tensor(y, "y").dtype:
             raise TypeError("h has y's type")
-        h_dtype = y.dtype
+        h_dtype = _tensor(y, "y").dtype
         yp = _check(y, "y", shape, h_dtype, device)
         y_stride = y.stride(0)
     elif h_dtype is None:
@@ -234,8 +260,8 @@ def norm_residual(x, y=None, *, post=None, pre=None, post_gamma=None, post_beta=
     x_stride = x.stride(0)
     if rows <= 1:  # the strides of single rows are never used
         x_stride = y_stride = xo_stride = h_stride = width
-    desc = _NORM_DESC.pack(
-        rows, width, stream_kind, branch_kind, _lookup(_NORMS, post, "post"), _lookup(_NORMS, pre, "pre"),
+    desc = _pack(
+        _NORM_DESC, rows, width, stream_kind, branch_kind, _lookup(_NORMS, post, "post"), _lookup(_NORMS, pre, "pre"),
         _lookup(_GATES, gate_act, "gate_act"), rows_per_cond, res_scale, branch_scale, eps, x_stride, y_stride,
         xo_stride, h_stride, cond_stride or 0)
     code = _native("kb_norm_residual")(desc, xp, yp, *affine, *cond, xo_p, h_p, _raw(stream, device))
@@ -270,7 +296,7 @@ def diff_attention(q, k, v, lam, *, gamma=None, out_scale=1.0, eps=1e-5, scale=N
     dtype = q.dtype
     if dtype is not torch.bfloat16 and dtype is not torch.float16:
         raise TypeError(f"q must be float16 or bfloat16, got {dtype}")
-    q_shape, k_shape = q.shape, k.shape
+    q_shape, k_shape = q.shape, _tensor(k, "k").shape
     if len(q_shape) != 5 or len(k_shape) != 5 or q_shape[3] != 2:
         raise ValueError("q and k must be [batch, tokens, heads, 2, d]")
     batch, q_len, heads, _, d = q_shape
@@ -284,7 +310,7 @@ def diff_attention(q, k, v, lam, *, gamma=None, out_scale=1.0, eps=1e-5, scale=N
     mp = mask_batch = 0
     if key_mask is not None:
         mp = _check(key_mask, "key_mask", (batch, kv_len),
-                    torch.bool if key_mask.dtype is torch.bool else torch.uint8, device)
+                    torch.bool if _tensor(key_mask, "key_mask").dtype is torch.bool else torch.uint8, device)
         mask_batch = key_mask.stride(0)
     if out is None:
         out = _empty(q, (batch, q_len, heads, 2 * d), dtype, stream, device)
@@ -292,8 +318,8 @@ def diff_attention(q, k, v, lam, *, gamma=None, out_scale=1.0, eps=1e-5, scale=N
     else:
         op = _check(out, "out", (batch, q_len, heads, 2 * d), dtype, device)
     qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
-    desc = _DIFF_DESC.pack(
-        _DTYPES[dtype], batch, q_len, kv_len, heads, kv_heads, d, bool(causal), window,
+    desc = _pack(
+        _DIFF_DESC, _DTYPES[dtype], batch, q_len, kv_len, heads, kv_heads, d, bool(causal), window,
         d**-0.5 if scale is None else scale, out_scale, eps, qs[0], qs[1], qs[2], qs[3], ks[0], ks[1], ks[2], ks[3],
         vs[0], vs[1], vs[2], os[0], os[1], os[2], mask_batch)
     sp = _status(status, device)
@@ -315,5 +341,5 @@ def diff_lambda(q1, k1, q2, k2, lambda_init):
         raise ValueError("the four vectors must have one shape [heads, d]")
     heads, d = vectors[0].shape
     lam = np.empty(heads, np.float32)
-    call("kb_diff_lambda", *[t.ctypes.data for t in vectors], heads, d, lambda_init, lam.ctypes.data)
+    call("kb_diff_lambda", *[t.ctypes.data for t in vectors], heads, d, float(lambda_init), lam.ctypes.data)
     return lam

@@ -182,3 +182,9 @@ def test_attention_takes_any_nested_output(kw):
              k_map=64, v_batch=4096, v_token=256, v_head=128, out_batch=4096, out_token=512, out_head=128)
     desc = _capi.DiffAttentionDesc(**{**d, **kw})
     assert _capi.load().kb_diff_attention_workspace(ctypes.byref(desc), ctypes.byref(need)) == _capi.KB_OK
+
+
+@pytest.mark.parametrize("init", [None, "half", [0.5, 0.5]])
+def test_diff_lambda_refuses_what_is_no_number(init):
+    with pytest.raises((TypeError, ValueError)):
+        block.diff_lambda(*[np.zeros((2, 4), np.float32)] * 4, init)

@@ -602,3 +602,39 @@ def test_rope_shows_non_finite_frequencies(cuda, dtype, head_dim, layout, shared
     cache = torch.full((4, 5, head_dim), 3.0, dtype=dtype, device="cuda")
     block.rope_axes(y, pos, freqs, cache, rotary_heads=3, layout=layout, slots=torch.tensor([2, -1, 9, 0], device="cuda"))
     assert (cache[[1, 3]] == 3).all() and torch.isnan(cache[[0, 2]][:, bad]).all() and not torch.isnan(cache[:, ~bad]).any()
+
+
+@pytest.mark.parametrize("kw", [dict(window=2**31), dict(window=-2**40), dict(window="wide"), dict(window=2.5), dict(scale=1e39),
+                                dict(eps="small"), dict(out_scale=None), dict(key_mask=[True]), dict(k=None), dict(v=3),
+                                dict(out=[0]), dict(gamma=2.0), dict(kv_lens=7)])
+def test_attention_arguments_of_no_use_are_refused(cuda, kw):
+    q, k, v, lam, _ = attn_inputs(2, 5, 8, 2, 2, 64, torch.bfloat16)
+    with pytest.raises((TypeError, ValueError, _capi.KbError)):
+        block.diff_attention(**{**dict(q=q, k=k, v=v, lam=lam, causal=True), **kw})
+
+
+@pytest.mark.parametrize("kw", [dict(rows_per_cond=2**31), dict(rows_per_cond="all"), dict(eps=None),
+                                dict(y=[1.0]), dict(x_out=3), dict(h="h"), dict(gate=1.0, rows_per_cond=4)])
+def test_norm_arguments_of_no_use_are_refused(cuda, kw):
+    x = torch.zeros(4, 96, device="cuda")
+    with pytest.raises((TypeError, ValueError, _capi.KbError)):
+        block.norm_residual(x, **{**dict(y=x, pre="rms"), **kw})
+
+
+@pytest.mark.parametrize("kw", [dict(rotary_heads=2**32 + 1), dict(rotary_heads=2.0), dict(rotary_heads=-(2**32) + 2),
+                                dict(freqs=None), dict(positions=[1]), dict(out=[0]), dict(slots=1, out=True)])
+def test_rope_arguments_of_no_use_are_refused(cuda, kw):
+    x, pos, freqs = rope_inputs(3, 2, 32, 16, 1, 1, torch.float32, 9)
+    if kw.get("out") is True:
+        kw = dict(kw, out=torch.empty_like(x))
+    with pytest.raises((TypeError, ValueError, _capi.KbError)):
+        block.rope_axes(**{**dict(x=x, positions=pos, freqs=freqs), **kw})
+
+
+def test_streams_of_no_use_are_refused(cuda):
+    q, k, v, lam, _ = attn_inputs(1, 2, 8, 2, 2, 64, torch.bfloat16)
+    for stream in ("side", 1.5, q):
+        with pytest.raises(TypeError):
+            block.diff_attention(q, k, v, lam, stream=stream)
+        with pytest.raises(TypeError):
+            block.norm_residual(q[0, 0, 0], pre="rms", stream=stream, h=torch.empty_like(q[0, 0, 0]), x_out=False)
