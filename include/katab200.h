@@ -474,6 +474,15 @@ KB_API int kb_test_wait_timeout(unsigned long long limit_ns, uint32_t* status, u
 KB_API int kb_test_int8_gemm_i32_wait_limit(const int8_t* a, const int8_t* w, int32_t* dots, int m, int n, int kp,
                                             unsigned long long wait_limit_ns, uint32_t* status, uintptr_t stream);
 
+/* kb_diff_attention (no gamma, lengths or mask) with the limit of its waits on
+ * work shortened to wait_limit_ns (1 ns .. 2 s): calls of many queries that
+ * take longer abort, record KB_STATUS_TIMEOUT in status[2] and return (out is
+ * then partial); those of few queries wait for nothing. */
+KB_API int kb_test_diff_attention_wait_limit(const kb_diff_attention_desc* desc, const uint16_t* q, const uint16_t* k,
+                                             const uint16_t* v, const float* lambda, uint16_t* out, void* workspace,
+                                             size_t workspace_bytes, unsigned long long wait_limit_ns,
+                                             uint32_t* status, uintptr_t stream);
+
 /* ------------------------------------------------------------------ model and evaluator */
 
 #define KB_PREC_INT8 0  /* W8A8: every trunk linear INT8 x INT8 -> INT32 */

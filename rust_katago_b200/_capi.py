@@ -52,6 +52,8 @@ SIGNATURES: dict[str, tuple] = {
     "kb_norm_residual": (I, [P, P, P, P, P, P, P, P, P, P, P, P, STREAM]),
     "kb_diff_attention_workspace": (I, [P, ctypes.POINTER(ctypes.c_size_t)]),
     "kb_diff_attention": (I, [P, P, P, P, P, P, P, P, P, P, ctypes.c_size_t, P, STREAM]),
+    "kb_test_diff_attention_wait_limit": (
+        I, [P, P, P, P, P, P, P, ctypes.c_size_t, ctypes.c_ulonglong, P, STREAM]),
     "kb_diff_lambda": (I, [P, P, P, P, I, I, F, P]),
     "kb_status_reset": (I, [P, STREAM]),
     "kb_mxfp8_dimensions": (I, [I, I, IP, IP, ctypes.POINTER(ctypes.c_size_t), ctypes.POINTER(ctypes.c_size_t)]),

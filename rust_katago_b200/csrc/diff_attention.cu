@@ -209,11 +209,12 @@ extern "C" int kb_diff_attention_workspace(const kb_diff_attention_desc* desc, s
   return KB_OK;
 }
 
-extern "C" int kb_diff_attention(const kb_diff_attention_desc* desc, const uint16_t* q, const uint16_t* k,
-                                 const uint16_t* v, const float* lambda, const float* gamma, const int32_t* kv_lens,
-                                 const uint8_t* key_mask, uint16_t* out, void* workspace, size_t workspace_bytes,
-                                 uint32_t* status, uintptr_t stream) {
-  using namespace kb;
+namespace kb {
+namespace {
+
+int run(const kb_diff_attention_desc* desc, const uint16_t* q, const uint16_t* k, const uint16_t* v, const float* lambda,
+        const float* gamma, const int32_t* kv_lens, const uint8_t* key_mask, uint16_t* out, void* workspace,
+        size_t workspace_bytes, uint32_t* status, uint32_t wait_limit_ns, uintptr_t stream) {
   const int rc = check_desc(desc);
   if (rc) return rc;
   const kb_diff_attention_desc& d = *desc;
@@ -241,8 +242,31 @@ extern "C" int kb_diff_attention(const kb_diff_attention_desc* desc, const uint1
     a.part_ml = static_cast<float2*>(workspace);
     a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + at);
   }
-  const int rc2 = p.few ? diff_decode_launch(a, p.splits, s) : diff_tc_launch(a, p.splits, status, s);
+  const int rc2 = p.few ? diff_decode_launch(a, p.splits, s) : diff_tc_launch(a, p.splits, status, wait_limit_ns, s);
   return rc2 || !need ? rc2 : diff_combine_launch(a, p.splits, s);
+}
+
+}  // namespace
+}  // namespace kb
+
+extern "C" int kb_diff_attention(const kb_diff_attention_desc* desc, const uint16_t* q, const uint16_t* k,
+                                 const uint16_t* v, const float* lambda, const float* gamma, const int32_t* kv_lens,
+                                 const uint8_t* key_mask, uint16_t* out, void* workspace, size_t workspace_bytes,
+                                 uint32_t* status, uintptr_t stream) {
+  return kb::run(desc, q, k, v, lambda, gamma, kv_lens, key_mask, out, workspace, workspace_bytes, status, 0, stream);
+}
+
+extern "C" int kb_test_diff_attention_wait_limit(const kb_diff_attention_desc* desc, const uint16_t* q,
+                                                 const uint16_t* k, const uint16_t* v, const float* lambda,
+                                                 uint16_t* out, void* workspace, size_t workspace_bytes,
+                                                 unsigned long long wait_limit_ns, uint32_t* status, uintptr_t stream) {
+  using namespace kb;
+  if (!status || wait_limit_ns == 0 || wait_limit_ns > 2000000000ull) {
+    set_error("kb_test_diff_attention_wait_limit: invalid arguments");
+    return KB_E_INVALID;
+  }
+  return run(desc, q, k, v, lambda, nullptr, nullptr, nullptr, out, workspace, workspace_bytes, status,
+             static_cast<uint32_t>(wait_limit_ns), stream);
 }
 
 extern "C" int kb_diff_lambda(const float* q1, const float* k1, const float* q2, const float* k2, int heads,

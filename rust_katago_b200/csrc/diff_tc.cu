@@ -42,6 +42,7 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "kb_diff.cuh"
 #include "kb_internal.h"
@@ -87,6 +88,7 @@ struct Geo {
 
 struct Items {
   int q_tiles, splits, count;
+  uint32_t wait_limit_ns;
   FastDiv by_splits, by_tiles, by_heads;  // by_tiles: causal calls by batch x heads
 };
 
@@ -187,8 +189,8 @@ __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
 
 // mbar_wait in few instructions (it is inlined some thirty times, and the
 // kernel's loops have to stay in the instruction cache), without a hint of how
-// long to suspend: the default wakes sooner.  The limit is two seconds of the
-// timer's low word.
+// long to suspend: the default wakes sooner.  The limit, two seconds or a test's
+// shorter one, is measured on the timer's low word.
 __device__ __forceinline__ bool try_wait(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
@@ -200,23 +202,25 @@ __device__ __forceinline__ bool try_wait(uint64_t* bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-__device__ __forceinline__ bool wait_short(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+__device__ __forceinline__ bool wait_short(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint32_t limit_ns) {
   if (try_wait(bar, parity)) return true;
   uint32_t t0, t1;
   asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t0));
 #pragma unroll 1
   while (!try_wait(bar, parity)) {
     asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t1));
-    if (t1 - t0 > static_cast<uint32_t>(kWaitLimitNs)) *abort_flag = 1;
+    if (t1 - t0 > limit_ns) *abort_flag = 1;
     if (*abort_flag) return false;
   }
   return true;
 }
 
 // The same for a whole warp, all lanes of which return what one would.
-#define KB_WARP_WAIT(bar, parity) __all_sync(0xffffffffu, wait_short(bar, parity, abort_flag))
+#define KB_WARP_WAIT(bar, parity) __all_sync(0xffffffffu, wait_short(bar, parity, abort_flag, limit_ns))
 
-template <int D, bool F16>
+// LIMITED: waits are limited to items.wait_limit_ns, for tests of what follows
+// when one runs out (a limit read from an argument costs the product 1%).
+template <int D, bool F16, bool LIMITED>
 __global__ void __launch_bounds__(kThreads, 1) diff_tc_kernel(const __grid_constant__ CUtensorMap map_q,
                                                               const __grid_constant__ CUtensorMap map_k,
                                                               const __grid_constant__ CUtensorMap map_v,
@@ -286,6 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1) diff_tc_kernel(const __grid_const
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const bool has_mask = a.key_mask != nullptr;
+  const uint32_t limit_ns = LIMITED ? items.wait_limit_ns : static_cast<uint32_t>(kWaitLimitNs);
 
   if (warp < kEpiWarp) {
     // ------------------------------------------------------------ softmax
@@ -585,8 +590,10 @@ __global__ void __launch_bounds__(kThreads, 1) diff_tc_kernel(const __grid_const
         const bool more = ws.valid;
         ok = issue_pv(0) && (!more || issue_s(0)) && issue_pv(1) && (!more || issue_s(1));
       }
-      if (__any_sync(0xffffffffu, *abort_flag) && elect_one()) {
-        int none = 0;  // let the MMAs issued so far finish before tensor memory goes
+      // Let the MMAs issued so far finish before tensor memory goes: whoever gives
+      // up a wait may do so when this warp is already through (else they are done).
+      if (elect_one()) {
+        int none = 0;
         tc_commit(drain);
         mbar_wait(drain, 0, &none);
       }
@@ -605,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, 1) diff_tc_kernel(const __grid_const
           tiles_of(a, items, b, qt, split, n, off, t0, t1);
           if (t0 >= t1) continue;
           const int hk = h / share, qb = busy & 1;
-          ok = wait_short(&q_empty[qb], ((busy >> 1) & 1) ^ 1, abort_flag);
+          ok = wait_short(&q_empty[qb], ((busy >> 1) & 1) ^ 1, abort_flag, limit_ns);
           if (!ok) break;
           mbar_arrive_expect_tx(&q_full[qb], 2 * G::kQk);
           for (int m = 0; m < 2; ++m)
@@ -615,14 +622,14 @@ __global__ void __launch_bounds__(kThreads, 1) diff_tc_kernel(const __grid_const
           for (int t = t0; t < t1; ++t) {
             const int stage = tile % kS;
             const uint32_t parity = ((tile / kS) & 1) ^ 1;
-            ok = wait_short(&k_empty[stage], parity, abort_flag);
+            ok = wait_short(&k_empty[stage], parity, abort_flag, limit_ns);
             if (!ok) break;
             mbar_arrive_expect_tx(&k_full[stage], 2 * G::kQk);
             for (int m = 0; m < 2; ++m)
               tma_load_5d(smem + G::kKOff + (stage * 2 + m) * G::kQk, &map_k, &k_full[stage], 0, t * kTile,
                           hk * bc.k_head, m * bc.k_map, b * bc.k_batch);
             ++tile;
-            ok = wait_short(&v_empty[stage], parity, abort_flag);
+            ok = wait_short(&v_empty[stage], parity, abort_flag, limit_ns);
             if (!ok) break;
             mbar_arrive_expect_tx(&v_full[stage], G::kV);
             for (int c = 0; c < static_cast<int>(G::kDv) / 64; ++c)
@@ -631,12 +638,11 @@ __global__ void __launch_bounds__(kThreads, 1) diff_tc_kernel(const __grid_const
             ++tile_v;
           }
         }
-        if (*abort_flag) {  // let the copies issued so far land before shared memory goes
-          int none = 0;
-          for (int u = busy > 2 ? busy - 2 : 0; u < busy; ++u) mbar_wait(&q_full[u & 1], (u >> 1) & 1, &none);
-          for (int u = tile > kS ? tile - kS : 0; u < tile; ++u) mbar_wait(&k_full[u % kS], (u / kS) & 1, &none);
-          for (int u = tile_v > kS ? tile_v - kS : 0; u < tile_v; ++u) mbar_wait(&v_full[u % kS], (u / kS) & 1, &none);
-        }
+        // Let the copies issued so far land before shared memory goes, likewise.
+        int none = 0;
+        for (int u = busy > 2 ? busy - 2 : 0; u < busy; ++u) mbar_wait(&q_full[u & 1], (u >> 1) & 1, &none);
+        for (int u = tile > kS ? tile - kS : 0; u < tile; ++u) mbar_wait(&k_full[u % kS], (u / kS) & 1, &none);
+        for (int u = tile_v > kS ? tile_v - kS : 0; u < tile_v; ++u) mbar_wait(&v_full[u % kS], (u / kS) & 1, &none);
       }
     } else if (warp == kHiddenWarp) {
       // ---------------------------------------------------------- hidden keys
@@ -717,9 +723,9 @@ int encode(CUtensorMap* map, const void* base, int width, int box, long tokens, 
   return encode_nd(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, base, 2 + more, dims, bytes, boxes, swz);
 }
 
-template <int D, bool F16>
-int launch(const DiffArgs& a, int splits, unsigned* status, cudaStream_t s) {
-  auto kern = diff_tc_kernel<D, F16>;
+template <int D, bool F16, bool LIMITED>
+int launch(const DiffArgs& a, int splits, unsigned* status, uint32_t wait_limit_ns, cudaStream_t s) {
+  auto kern = diff_tc_kernel<D, F16, LIMITED>;
   int dev = 0;
   cudaGetDevice(&dev);
   static std::atomic<uint64_t> configured{0};
@@ -753,6 +759,7 @@ int launch(const DiffArgs& a, int splits, unsigned* status, cudaStream_t s) {
   Items it;
   it.q_tiles = (d.q_len + kTile - 1) / kTile;
   it.splits = splits;
+  it.wait_limit_ns = wait_limit_ns;
   const int64_t count = static_cast<int64_t>(d.batch) * d.heads * it.q_tiles * splits;
   if (count > 0x7fffffff - 65536 || static_cast<int64_t>(d.batch) * d.heads > 0x3fffffff) {
     set_error("kb_diff_attention: too many query tiles");
@@ -769,10 +776,15 @@ int launch(const DiffArgs& a, int splits, unsigned* status, cudaStream_t s) {
 
 }  // namespace
 
-int diff_tc_launch(const DiffArgs& a, int splits, unsigned* status, cudaStream_t s) {
+int diff_tc_launch(const DiffArgs& a, int splits, unsigned* status, uint32_t wait_limit_ns, cudaStream_t s) {
   const bool f16 = a.d.dtype == KB_DT_F16;
-  if (a.d.head_dim == 64) return f16 ? launch<64, true>(a, splits, status, s) : launch<64, false>(a, splits, status, s);
-  return f16 ? launch<32, true>(a, splits, status, s) : launch<32, false>(a, splits, status, s);
+  auto run = [&](auto limited) {
+    constexpr bool L = decltype(limited)::value;
+    if (a.d.head_dim == 64)
+      return f16 ? launch<64, true, L>(a, splits, status, wait_limit_ns, s) : launch<64, false, L>(a, splits, status, wait_limit_ns, s);
+    return f16 ? launch<32, true, L>(a, splits, status, wait_limit_ns, s) : launch<32, false, L>(a, splits, status, wait_limit_ns, s);
+  };
+  return wait_limit_ns ? run(std::true_type{}) : run(std::false_type{});
 }
 
 }  // namespace kb

@@ -116,7 +116,8 @@ __device__ __forceinline__ void write_partial(const DiffArgs& a, int splits, int
 constexpr int kMostCluster = 8;
 
 int diff_decode_launch(const DiffArgs& a, int splits, cudaStream_t s);
-int diff_tc_launch(const DiffArgs& a, int splits, unsigned* status, cudaStream_t s);
+// wait_limit_ns: a test's limit of its waits on work (0: kWaitLimitNs).
+int diff_tc_launch(const DiffArgs& a, int splits, unsigned* status, uint32_t wait_limit_ns, cudaStream_t s);
 int diff_combine_launch(const DiffArgs& a, int splits, cudaStream_t s);
 int smem_opt_in(const void* kernel, int bytes);
 

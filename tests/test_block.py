@@ -188,3 +188,11 @@ def test_attention_takes_any_nested_output(kw):
 def test_diff_lambda_refuses_what_is_no_number(init):
     with pytest.raises((TypeError, ValueError)):
         block.diff_lambda(*[np.zeros((2, 4), np.float32)] * 4, init)
+
+
+@pytest.mark.parametrize("limit,status", [(0, P), (2_000_000_001, P), (5, 0)])
+def test_wait_limits_of_no_use_are_refused(limit, status):
+    d = 64
+    desc = _capi.DiffAttentionDesc(dtype=_capi.DT_BF16, batch=1, q_len=1, kv_len=1, heads=1, kv_heads=1, head_dim=d,
+                                   scale=1.0, out_scale=1.0, q_map=d, k_map=d)
+    invalid(_capi.load().kb_test_diff_attention_wait_limit(ctypes.byref(desc), P, P, P, P, 2 * P, 0, 0, limit, status, 0))

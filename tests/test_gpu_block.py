@@ -5,6 +5,8 @@ an ulp of the 16-bit type relative to the value (2^-8 for bfloat16, 2^-11 for
 binary16 plus half its smallest subnormal), e = 2^-24 that of fp32.
 """
 
+import ctypes
+
 import pytest
 import torch
 
@@ -638,3 +640,33 @@ def test_streams_of_no_use_are_refused(cuda):
             block.diff_attention(q, k, v, lam, stream=stream)
         with pytest.raises(TypeError):
             block.norm_residual(q[0, 0, 0], pre="rms", stream=stream, h=torch.empty_like(q[0, 0, 0]), x_out=False)
+
+
+@pytest.mark.parametrize("limit_ns", [1, 3_000, 20_000])
+@pytest.mark.parametrize("q_len,kv_len,heads,d,dtype", [
+    (4096, 4096, 4, 64, torch.bfloat16), (4096, 4096, 4, 32, torch.float16), (256, 300_000, 2, 64, torch.float16)])
+def test_waits_that_run_out_are_reported_and_leave_the_device_usable(cuda, limit_ns, q_len, kv_len, heads, d, dtype):
+    q, k, v, lam, _ = attn_inputs(1, q_len, kv_len, heads, heads, d, dtype)
+    ref = block.diff_attention(q, k, v, lam, causal=True)
+    out = torch.empty_like(ref)
+    desc = _capi.DiffAttentionDesc(
+        dtype=block._DTYPES[dtype], batch=1, q_len=q_len, kv_len=kv_len, heads=heads, kv_heads=heads, head_dim=d, causal=1,
+        scale=d**-0.5, out_scale=1.0, eps=1e-5, q_token=q.stride(1), q_head=q.stride(2), q_map=d, k_token=k.stride(1),
+        k_head=k.stride(2), k_map=d, v_token=v.stride(1), v_head=v.stride(2), out_token=out.stride(1), out_head=out.stride(2))
+    need = ctypes.c_size_t()
+    _capi.call("kb_diff_attention_workspace", ctypes.byref(desc), ctypes.byref(need))
+    work = torch.zeros(max(need.value, 1), dtype=torch.uint8, device="cuda")
+
+    def run(limit):
+        status = torch.tensor([0, -1], dtype=torch.int32, device="cuda")
+        _capi.call("kb_test_diff_attention_wait_limit", ctypes.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                   lam.data_ptr(), out.data_ptr(), work.data_ptr(), need.value, limit, status.data_ptr(),
+                   torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        return status.tolist()
+
+    assert run(limit_ns) == [_capi.STATUS_TIMEOUT, -1]  # items of 30 tiles and more take 60 us and more
+    # shared and tensor memory of every SM are free again, nothing is in flight
+    for _ in range(2):
+        assert run(2_000_000_000) == [0, -1] and torch.equal(out, ref)
+        assert torch.equal(block.diff_attention(q, k, v, lam, causal=True), ref)
