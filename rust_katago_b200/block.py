@@ -289,8 +289,11 @@ def diff_attention(q, k, v, lam, *, gamma=None, out_scale=1.0, eps=1e-5, scale=N
     [batch, kv_len]); causal puts the queries at the end of the sequence (of
     kv_lens[b] tokens, of which k and v may hold only the first kv_len), window
     keeps the last `window` positions of each.  Queries that see no key give zeros.
-    status: a status word (int32 or uint32 [flags, first_layer], two elements).
-    Returns out [batch, q_len, heads, 2 d].
+    status: a status word (int32 or uint32 [flags, first_layer], two elements),
+    zero flags and first_layer -1 to begin with; a kernel that gives up one of its
+    waits (two seconds: a fault) sets KB_STATUS_TIMEOUT there and leaves out
+    partial, and without a status word nothing tells.  Returns out [batch, q_len,
+    heads, 2 d].
     """
     device = _device(q, "q")
     dtype = q.dtype

@@ -50,7 +50,10 @@ class Cache:
 class DiffBlock:
     """One block's weights: bf16 wqkv [(2 heads + 4 kv_heads) * d, width] ([Q | K | V], a head's two maps side by
     side, values 2 d wide), wout [width, heads * 2 d]; fp32 freqs [2 heads + 2 kv_heads, d / 2, axes], lam [heads],
-    sub_gamma [2 d], pre_gamma, post_gamma [width]; bf16 gate [1, width]."""
+    sub_gamma [2 d], pre_gamma, post_gamma [width]; bf16 gate [1, width].
+
+    status (int32 [flags, first_layer], on the device) is sticky: a flag says that a kernel of some call gave up a wait
+    and that its results are partial.  :meth:`check` reads it."""
 
     def __init__(self, heads: int, kv_heads: int, wqkv, wout, freqs, lam, sub_gamma, pre_gamma, post_gamma, gate,
                  lambda_init: float, eps: float = 1e-6):
@@ -60,6 +63,12 @@ class DiffBlock:
         self.q_freqs, self.k_freqs = freqs[: 2 * heads].contiguous(), freqs[2 * heads:].contiguous()
         self.pre_gamma, self.post_gamma, self.gate = pre_gamma, post_gamma, gate
         self.out_scale, self.eps = 1.0 - lambda_init, eps
+        self.status = torch.tensor([0, -1], dtype=torch.int32, device=wqkv.device)
+
+    def check(self) -> None:
+        """Raise RuntimeError if a kernel of an earlier call gave up a wait (waits for the calls on the current stream)."""
+        if flags := int(self.status[0]):
+            raise RuntimeError(f"a kernel of the block did not finish (status flags {flags})")
 
     @classmethod
     def random(cls, width: int, heads: int, kv_heads: int, head_dim: int, axes: int = 3, depth: int = 0, seed: int = 0):
@@ -98,7 +107,8 @@ class DiffBlock:
                         out=cache.rows, slots=cache.slots(new))
         cache.lens += new
         a = block.diff_attention(q.view(batch, new, self.heads, 2, d), cache.k, cache.v, self.lam, gamma=self.sub_gamma,
-                                 out_scale=self.out_scale, causal=causal, kv_lens=cache.lens, key_mask=key_mask)
+                                 out_scale=self.out_scale, causal=causal, kv_lens=cache.lens, key_mask=key_mask,
+                                 status=self.status)
         y = self._linear(a.view(rows, -1), self.wout)
         out, h = block.norm_residual(
             flat, y, post="rms", post_gamma=self.post_gamma, gate=self.gate, rows_per_cond=rows, pre="rms",
@@ -130,6 +140,7 @@ def main() -> None:
     for step in range(4):
         pos = torch.tensor([[boards], [0], [step]], dtype=torch.int32, device="cuda").repeat(1, batch)
         x, _ = net(torch.randn(batch, 1, 768, device="cuda").bfloat16(), pos, cache)
+    net.check()
     print(f"one token at a time: {tuple(x.shape)}, cache at {cache.lens.tolist()}, mean square {x.float().square().mean():.3f}")
 
 

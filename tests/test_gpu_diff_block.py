@@ -117,3 +117,17 @@ def test_calls_without_tokens_do_nothing(cuda, batch, new):
     x = torch.zeros(batch, new, 384, dtype=torch.bfloat16, device="cuda")
     out, h = net(x, torch.zeros(3, batch * new, dtype=torch.int32, device="cuda"), cache)
     assert out.shape == h.shape == (batch, new, 384) and cache.lens.tolist() == [0] * batch
+
+
+def test_kernels_that_do_not_finish_show(cuda, monkeypatch):
+    net = diff_block.DiffBlock.random(384, 6, 6, 32, seed=10)
+    seen = []
+    attention = diff_block.block.diff_attention
+    monkeypatch.setattr(diff_block.block, "diff_attention", lambda *a, **kw: seen.append(kw["status"]) or attention(*a, **kw))
+    net(torch.zeros(1, 2, 384, dtype=torch.bfloat16, device="cuda"), torch.zeros(3, 2, dtype=torch.int32, device="cuda"),
+        diff_block.Cache(1, 4, 6, 32))
+    assert seen[0] is net.status and net.status.tolist() == [0, -1]
+    net.check()
+    net.status[0] = 32  # what a kernel leaves that gave up a wait
+    with pytest.raises(RuntimeError):
+        net.check()
