@@ -48,9 +48,9 @@ assert _DIFF_DESC.size == ctypes.sizeof(_capi.DiffAttentionDesc)
 
 
 # What torch.cuda.current_device() and current_stream().cuda_stream return, without
-# the 10 us of their wrappers.
-_current_device = torch._C._cuda_getDevice
-_current_stream = torch._C._cuda_getCurrentRawStream
+# the 10 us of their wrappers (through those where a torch names them otherwise).
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def _raw(stream, device):

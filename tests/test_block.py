@@ -196,3 +196,18 @@ def test_wait_limits_of_no_use_are_refused(limit, status):
     desc = _capi.DiffAttentionDesc(dtype=_capi.DT_BF16, batch=1, q_len=1, kv_len=1, heads=1, kv_heads=1, head_dim=d,
                                    scale=1.0, out_scale=1.0, q_map=d, k_map=d)
     invalid(_capi.load().kb_test_diff_attention_wait_limit(ctypes.byref(desc), P, P, P, P, 2 * P, 0, 0, limit, status, 0))
+
+
+def test_wrappers_load_without_torch_private_names(monkeypatch):
+    import importlib.util
+
+    import torch
+
+    for name in ("_cuda_getDevice", "_cuda_getCurrentRawStream"):
+        monkeypatch.delattr(torch._C, name, raising=False)
+    spec = importlib.util.spec_from_file_location("rust_katago_b200._block_copy", block.__file__)
+    copy = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(copy)
+    assert copy._current_device is torch.cuda.current_device and callable(copy._current_stream)
+    with pytest.raises(ValueError):
+        copy.norm_residual(torch.zeros(1, 8))
