@@ -15,8 +15,9 @@ Tensors may have any strides as long as the innermost dimension is contiguous
 current stream of the tensors' device, or to ``stream``; outputs and scratch
 that a call allocates belong to that stream.  Wrong arguments raise
 ``ValueError`` / ``TypeError`` here or :class:`rust_katago_b200._capi.KbError`
-from the library.  No reference counterparts: the reference's trunk has one
-softmax map over 361 tokens.
+from the library.  Inference only: nothing is recorded for autograd, and the
+outputs carry no gradient even where an input requires one.  No reference
+counterparts: the reference's trunk has one softmax map over 361 tokens.
 """
 
 from __future__ import annotations
@@ -151,7 +152,8 @@ def rope_axes(x, positions, freqs, out=None, *, rotary_heads=None, layout="pairs
     heads from rotary_heads on (default: none) and elements from 2 * pairs on
     are copied.  layout: "pairs" mixes (2p, 2p + 1), "halves" (p, p + pairs).
     With slots (int64 [tokens]) token t goes to row slots[t] of out [rows,
-    heads, head_dim] (a cache), rows outside it are skipped.  Returns out.
+    heads, head_dim] (a cache), rows outside it are skipped (two tokens with one
+    slot: either may stay).  A NaN or infinite frequency makes its pair NaN.  Returns out.
     """
     device = _device(x, "x")
     dtype, shape = x.dtype, x.shape
