@@ -670,3 +670,59 @@ def test_waits_that_run_out_are_reported_and_leave_the_device_usable(cuda, limit
     for _ in range(2):
         assert run(2_000_000_000) == [0, -1] and torch.equal(out, ref)
         assert torch.equal(block.diff_attention(q, k, v, lam, causal=True), ref)
+
+
+def both_operators(g):
+    """Calls of the rotary operator and of the norms on inputs of their own: run(stream) -> tensors."""
+    x, pos, freqs = rope_inputs(500, 6, 64, 32, 3, 1, torch.bfloat16, 300, seed=21)
+    s, y = (torch.randn(700, 768, generator=g, device="cuda") for _ in range(2))
+    gate = torch.randn(70, 768, generator=g, device="cuda").bfloat16()
+
+    def run(stream=None):
+        return (block.rope_axes(x, pos, freqs, stream=stream),
+                *block.norm_residual(s, y.bfloat16() if stream is None else yb, post="rms", pre="layer", gate=gate,
+                                     rows_per_cond=10, stream=stream))
+
+    yb = y.bfloat16()
+    return run, (x, s, yb)
+
+
+def test_rope_and_norms_repeat_on_any_stream_and_in_graphs(cuda):
+    run, inputs = both_operators(torch.Generator(device="cuda").manual_seed(20))
+    ref = run()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    outs = [run(side), run(side.cuda_stream)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = run(torch.cuda.current_stream())
+    graph.replay()
+    for got in (*outs, captured):
+        assert all(torch.equal(a, b) for a, b in zip(got, ref))
+    for t in inputs:
+        t.mul_(0.5)
+    graph.replay()
+    for a, b in zip(captured, run(torch.cuda.current_stream())):
+        assert torch.equal(a, b)
+
+
+def test_rope_and_norm_offsets_past_32_bits(cuda):
+    step = (1 << 25) + 264
+    room = torch.empty(160 * step, dtype=torch.bfloat16, device="cuda")
+    x, pos, freqs = rope_inputs(160, 4, 64, 32, 2, 4, torch.bfloat16, 99, seed=22)
+    far, to = (room.as_strided((160, 4, 64), (step, 64, 1), at) for at in (0, 256))
+    far.copy_(x)
+    ref = block.rope_axes(x, pos, freqs)
+    assert torch.equal(block.rope_axes(far, pos, freqs), ref)
+    assert torch.equal(block.rope_axes(x, pos, freqs, out=to), ref)
+    slots = torch.arange(159, -1, -1, device="cuda")
+    assert torch.equal(block.rope_axes(x, pos, freqs, out=to, slots=slots), ref.flip(0))
+    kw = dict(post="rms", pre="layer", gate=x[:16].flatten(1), rows_per_cond=10)
+    y = ref.flatten(1)
+    fx, fy = (room.as_strided((160, 256), (step, 1), at) for at in (0, 1024))
+    fy.copy_(y)
+    a = block.norm_residual(x.flatten(1), y, **kw)
+    b = block.norm_residual(fx, fy, x_out=room.as_strided((160, 256), (step, 1), 2048),
+                            h=room.as_strided((160, 256), (step, 1), 4096), **kw)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
