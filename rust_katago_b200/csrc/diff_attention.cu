@@ -77,7 +77,12 @@ __global__ void __launch_bounds__(32 * kJoinWarps) diff_combine_kernel(const Dif
 // of one of the latter (32 sequences of 2,000 keys: 20 queries 64 against 42 us,
 // 8 queries of 4 grouped heads 107 against 261 us), so the sums of tiles decide.
 // A call of few tiles and short keys is all latency, where the former is quicker
-// (120 queries on 1,000 keys, 4 heads: 15 against 22 us).
+// as long as its clusters fit one wave (one sequence of 1,000 keys: 32 tiles, 120
+// queries of 4 heads, 14 against 21 us; 36 tiles, 96 queries of 6, 24 against 22;
+// 48 tiles, 128 queries of 6, 26 and 26; 361 queries and keys: 23 tiles, 1 head, 11
+// against 13, 46 tiles, 2 heads, 12 against 14, 138 tiles, 6 heads, 15 against 14).
+// With longer keys it is not (24 tiles on 4,096 keys, 64 queries of 6 heads, 22
+// against 21; 36 tiles on 2,048 keys 29 against 23).
 struct Plan {
   bool few = false;
   int splits = 1;
@@ -114,8 +119,11 @@ Plan make_plan(const kb_diff_attention_desc& d) {
     p.joined = p.splits <= kMostCluster;
   } else {
     // Parts of the keys so that the items fill the SMs evenly: rounds of items
-    // times an item's time, plus the join, in microseconds as measured (a tile
-    // of 128 keys 2, an item's start and end 2.5, the join 4 and its bytes).
+    // times an item's time, plus the join, in microseconds (a tile of 128 keys
+    // 2, as the prompt takes; an item's start and end 2.5, the join 4 and its
+    // bytes, fitted to the order of the choices: the times themselves come out
+    // low where parts are short, 119 for 361 tokens on three 16,001-key caches
+    // that take 148).
     const int64_t tiles = (keys + kTileKeys - 1) / kTileKeys, sms = num_sms(dev);
     const int64_t units = static_cast<int64_t>(d.batch) * many_tiles;
     const double part_bytes = static_cast<double>(d.batch) * d.q_len * d.heads * 32.0 * d.head_dim;

@@ -22,8 +22,8 @@
 // by 2^8, so most steps skip the reduction over keys and the rescaling.
 //
 // Measured: one token each of 64 sequences on caches of 4,096 to 8,192 keys, 12
-// heads of 64 on 4 key/value heads, bf16: 132 us, 6.1 TB/s (0.94 of the copy
-// rate); one token on 1,083 keys, 6 heads: 8 us, launch and latency.
+// heads of 64 on 4 key/value heads, bf16: 132 us in a graph, 6.1 TB/s (0.94 of the
+// copy rate), 142 a call; one token on 1,083 keys, 6 heads: 8 us, launch and latency.
 // Keys are split over blocks and within a block over its warps.  The warps'
 // parts are joined in shared memory; the blocks' parts through distributed
 // shared memory when the blocks of a tile form a cluster (up to eight: one

@@ -31,7 +31,7 @@
 // and diff_combine joins the parts in a fixed order.
 //
 // Measured: 8,192-token causal prompt, 12 heads of 64 on 4 key/value heads, bf16:
-// 360 us (0.86 PFLOP/s, 0.51 of the measured GEMM rate) at 970 to 990 W of the
+// 350 to 360 us (0.87 PFLOP/s, 0.52 of the measured GEMM rate) at 970 to 990 W of the
 // 1,000 W cap.  A tile of 128 keys of both maps takes about 3,400 clocks, of
 // which its exponentials are 2,048 of the special-function unit and its products
 // 1,536 of the tensor pipe.  What bounds it is the chain of one map: scores from
@@ -53,7 +53,9 @@ namespace kb {
 namespace {
 
 constexpr int kTile = 128;  // queries per item, keys per tile
-constexpr int kFirst = 96;  // keys of the first of the two parts of P
+// Keys of the first of the two parts of P (32 / 64 / 96: that prompt 361 / 347 /
+// 355 us, 361 tokens on three 16,001-key caches 154 / 149 / 149: alike from 64 on).
+constexpr int kFirst = 96;
 constexpr int kThreads = 512;
 constexpr int kEpiWarp = 8, kMmaWarp = 12, kLoadWarp = 13, kHiddenWarp = 14;
 constexpr uint32_t kTmemCols = 512;

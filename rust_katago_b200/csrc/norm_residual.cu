@@ -17,8 +17,8 @@
 // error to h.
 // Measured: 92,416 x 768 bf16 with a gate row per 361 rows 99 us, 5.7 TB/s (0.88
 // of the copy rate); 8,191 x 5,120, fp32 stream and bf16 branch, layer norms 100
-// us, 5.0 TB/s (block-wide sums between loads); 20,000 x 1,001 bf16, single
-// elements, 81 us.
+// us, 5.0 TB/s (block-wide sums between loads); 20,000 rows of bf16 RMS norms by
+// single elements, 1,001 columns 61 us (1,000 by eights 34), 4,099 columns 322.
 #include <stdint.h>
 
 #include <atomic>
@@ -38,9 +38,15 @@ struct NormArgs {
   void *x_out, *h;
 };
 
-// Runs of rows per resident group (one leaves SMs idle at the end, 111 instead of
-// 99 us for 92,416 x 768; four or more build the shared vectors too often), and
-// groups of one warp that an SM holds, by chunks per thread.
+// Runs of rows per resident group (one leaves SMs idle at the end, 109 instead of
+// 99 us for 92,416 x 768 with a gate per 361 rows; four build the shared vectors
+// too often, 101 us, and 128 instead of 112 for 60,000 x 1,024 layer norms), and
+// groups of one warp to plan for on an SM, by chunks per thread: they set the
+// length of the runs, not what an SM holds (with four chunks and both shifts its
+// shared memory has room for 13).  One and two chunks, 12 / 20 / 28: 92,416 x 512
+// 76 / 66 / 67 us, 92,416 x 256 layer norms of fp32 61 / 58 / 58.  Three and four,
+// 8 / 12 / 16 / 20: 92,416 x 768 RMS with gates 109 / 105 / 99 / 102, layer norms
+// 131 / 99 / 104 / 110, 60,000 x 1,024 layer norms with gates 105 / 108 / 112 / 114.
 constexpr int kRunsPerSlot = 2;
 constexpr int kResident1 = 20, kResident2 = 20, kResident3 = 16;
 

@@ -13,9 +13,9 @@
 // 2^-32 of a turn, exact for long positions where fp32 is not (position 30,000
 // times a frequency of 1 costs fp32 1e-3).  (In fp64 the conversions bounded
 // the kernel: 92,416 tokens of 36 x 64 bf16 took 195 us.)
-// Measured: that case 162 us, 5.25 TB/s (0.80 of the copy rate), bound by the
-// bytes that 480 threads of 128 registers keep in flight; 32,845 tokens of 12 x 32
-// fp32, three axes, 25 us, 4.0 TB/s.
+// Measured: that case 160 us, 5.3 TB/s (0.81 of the copy rate), bound by the
+// bytes that 480 threads of 126 registers keep in flight; 32,845 tokens of 12 x 32
+// fp32, three axes, 25 us, 4.1 TB/s.
 #include <math.h>
 #include <stdint.h>
 
